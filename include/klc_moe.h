@@ -28,6 +28,8 @@
  *   klc_locality_route       <- route()'s locality steps: _apply_locality_bias :331-363,
  *                               _guarded_expert_selection :365-394, predict_experts :426-440,
  *                               _update_sticky_scores / _update_workload_scores :396-424
+ *   klc_attn_*, klc_rope_append <- StreamedAttention.forward        streamed_attention.py:100-152
+ *   klc_kv_*                 <- KVCacheManager                  kv_cache_manager.py:23-113
  *   klc_runtime_dequant      <- RuntimeDequantizer.dequantize   runtime_dequantizer.py:30-52
  *                               (unpack_lowbit adaptive_quantizer.py:183-213,
  *                                reconstruct_pruned tensor_pruner.py:62-69)
@@ -430,6 +432,50 @@ int klc_locality_route(const klc_locality_config* cfg, const uint16_t* logits, i
                        const uint8_t* resident, int64_t resident_stride, void* state, size_t state_bytes,
                        int32_t* out_experts, uint16_t* out_w, int32_t* out_raw, int32_t* out_pred, int32_t* out_npred,
                        uint8_t* out_flags, void* stream);
+
+/* ---- attention -----------------------------------------------------------
+ * The attention half of the executor's layer (StreamedAttention.forward,
+ * streamed_attention.py:100-152: grouped heads, sinks, sliding window) for
+ * batches of sequences.  Elements are bf16 or f16 (KLC_BF16 / KLC_F16), head
+ * width D is 64 or 128, and query head h reads key head h / (heads / kv_heads)
+ * (at most 64 query heads per key head).  Scores, softmax statistics and sums
+ * are fp32; the softmax numerators are rounded to the element type for the
+ * product with the values, and the output once at the end.  window 0 sees all
+ * earlier keys, window w the last w (the own key among them).  sinks: fp32
+ * [heads] or NULL, one more logit per head (unscaled) that takes part in the
+ * denominator only.  A row that sees no key gives zeros, and -inf (or the
+ * sink) as its log-sum-exp.
+ *
+ * `status`: a device buffer of klc_status_bytes that the caller zeroed once
+ * (or NULL).  The first device-side fault is recorded in it
+ * (klc_workspace_status reads it; zero it to go on); a row with a fault gets
+ * an unspecified output, and nothing outside the tensors is read or written. */
+typedef struct klc_attn_dims {
+  int32_t dtype;    /* enum klc_dtype: KLC_BF16 or KLC_F16 */
+  int32_t heads;    /* query heads  */
+  int32_t kv_heads; /* key heads    */
+  int32_t head_dim; /* 64 or 128    */
+  int32_t window;   /* 0: none      */
+  float scale;      /* > 0          */
+} klc_attn_dims;
+int klc_status_bytes(size_t* out_bytes);
+
+/* Causal attention over whole prompts, packed: sequence b has the query rows
+ * cu_q[b] .. cu_q[b+1] of q [q_tokens, heads, D] and the key rows cu_k[b] ..
+ * cu_k[b+1] of k and v [k_tokens, kv_heads, D] (int32 offsets on the device,
+ * ascending; cu_q may be passed for both).  The last query row sees the last
+ * key: with more keys than queries the first keys are an earlier part of the
+ * sequence.  Token and head strides are in elements, multiples of 8; rows are
+ * 16-byte aligned.  lse fp32 [q_tokens, heads] or NULL.  Rows of q past
+ * cu_q[batch] are not written.  A non-finite value row of a sequence's own
+ * keys may reach up to 127 rows before it.  Offsets that leave the tensors are
+ * recorded as KLC_ERR_DEVICE_FAULT and the sequence is skipped.  Replaces
+ * StreamedAttention.forward's loop over the tokens of a prompt.             */
+int klc_attn_prompt(const klc_attn_dims* dims, const void* q, int64_t q_tokens, int64_t q_token_stride,
+                    int64_t q_head_stride, const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                    int64_t v_token_stride, int64_t v_head_stride, int64_t k_tokens, const int32_t* cu_q,
+                    const int32_t* cu_k, int64_t batch, const float* sinks, void* out, int64_t out_token_stride,
+                    int64_t out_head_stride, float* lse, void* status, void* stream);
 
 /* ---- expert parallelism over NVLink peer memory ------------------------
  * No counterpart in the reference (one process, one device): the node-level

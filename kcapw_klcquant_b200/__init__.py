@@ -4,12 +4,15 @@ Drop-in modules mirror the reference's (klcquant) module names:
 ``streamed_moe_router``, ``mxfp4_expert``, ``runtime_dequantizer``.  All MoE
 math runs in the CUDA kernels of ``libklcmoe.so`` (C ABI in include/klc_moe.h).
 """
+from .attention import attn_prompt, check_device_status
 from .mxfp4_expert import FP4_VALUES, ExpertCacheStats, Mxfp4ExpertStore, PackedLayer, dequantize_mxfp4_matrix
 from .moe import MoeLayer, RouteBatch, rms_norm
 from .runtime_dequantizer import QuantizedTensorMeta, RuntimeDequantizer, parse_bool
 from .streamed_moe_router import RouterStats, RoutingLocalityConfig, StreamedMoERouter
 
 __all__ = [
+    "attn_prompt",
+    "check_device_status",
     "FP4_VALUES",
     "ExpertCacheStats",
     "Mxfp4ExpertStore",

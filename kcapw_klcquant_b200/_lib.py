@@ -106,6 +106,17 @@ class KlcWeights(ctypes.Structure):
     ]
 
 
+class KlcAttnDims(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32),
+        ("heads", c_int32),
+        ("kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("window", c_int32),
+        ("scale", c_float),
+    ]
+
+
 # name -> argtypes (every entry point returns int, except klc_last_error)
 SIGNATURES: dict[str, list] = {
     "klc_version": [],
@@ -171,6 +182,10 @@ SIGNATURES: dict[str, list] = {
     "klc_ep_status": [c_void_p, c_void_p, POINTER(c_int), POINTER(c_int), c_void_p],
     "klc_ep_received_rows": [c_void_p, POINTER(c_int64), c_void_p],
     "klc_ep_destroy": [c_void_p],
+    "klc_status_bytes": [POINTER(c_size_t)],
+    "klc_attn_prompt": [POINTER(KlcAttnDims), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                        c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                        c_void_p],
     "klc_rms_norm": [c_void_p, c_void_p, c_int64, c_int64, c_float, c_void_p, c_void_p],
     "klc_runtime_dequant": [c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int64, c_void_p, c_int, c_void_p],
 }
@@ -198,7 +213,7 @@ def lib() -> ctypes.CDLL:
     h.klc_last_error.argtypes = []
     h.klc_last_error.restype = c_char_p
     # the structures passed by pointer must have the library's layout
-    for which, struct in enumerate((KlcDims, KlcWeights, KlcLocalityConfig, KlcNextRouter)):
+    for which, struct in enumerate((KlcDims, KlcWeights, KlcLocalityConfig, KlcNextRouter, KlcAttnDims)):
         n = c_size_t(0)
         if h.klc_struct_size(which, ctypes.byref(n)) != KLC_OK or n.value != ctypes.sizeof(struct):
             raise ImportError(f"{LIB_PATH} was built with another {struct.__name__} layout ({n.value} B) than this "

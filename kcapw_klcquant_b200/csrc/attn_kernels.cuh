@@ -1,0 +1,40 @@
+// Launch parameters and internal entry points of the attention kernels.
+#pragma once
+
+#include <cuda.h>
+
+#include "klc_common.cuh"
+
+namespace klc {
+namespace attn {
+
+// tensor-core kernel (attn_tc.cu): prompts, and the shared prefix of decode rows
+struct TcParams {
+  const int32_t* cu_q;  // [batch + 1] first query row of each sequence (or group of rows)
+  const int32_t* cu_k;  // prompts: [batch + 1] first key row
+  int batch;
+  int64_t total_q, total_k;
+  int heads, group, tpt;  // query heads; per key head; tokens per row tile
+  float scale_log2;       // scale * log2(e)
+  int window;
+  const float* sinks;
+  void* out;
+  int64_t out_ts, out_hs;
+  float* lse;
+  DeviceStatus* status;
+  // prefix of decode rows
+  const int32_t* prefix_lens;  // [batch]
+  const int32_t* lens;         // [total_q]
+  const int32_t* block_table;
+  int64_t table_stride, pages;
+  int page_size;
+  float* part_o;    // [splits][total_q][heads][D]
+  float2* part_ml;  // [splits][total_q][heads]
+};
+
+// K or V pool [pages][kv_heads][page_size][D] (page stride in elements), box of box_rows x 64
+int pool_map(CUtensorMap* m, int dtype, int head_dim, const void* base, int64_t pages, int kv_heads, int page_size,
+             int64_t page_stride, int box_rows);
+
+}  // namespace attn
+}  // namespace klc

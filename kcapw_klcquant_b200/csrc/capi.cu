@@ -48,6 +48,12 @@ extern "C" int klc_capabilities(int* flags) {
   return KLC_OK;
 }
 
+extern "C" int klc_status_bytes(size_t* out_bytes) {
+  if (out_bytes == nullptr) return klc::fail(KLC_ERR_INVALID, "klc_status_bytes: null output");
+  *out_bytes = sizeof(klc::DeviceStatus);
+  return KLC_OK;
+}
+
 extern "C" int klc_device_sm_count(int* out_sms) {
   if (out_sms == nullptr) return klc::fail(KLC_ERR_INVALID, "klc_device_sm_count: null output");
   int dev = 0;
@@ -103,6 +109,7 @@ extern "C" int klc_struct_size(int which, size_t* out_bytes) {
     case 1: *out_bytes = sizeof(klc_moe_weights); return KLC_OK;
     case 2: *out_bytes = sizeof(klc_locality_config); return KLC_OK;
     case 3: *out_bytes = sizeof(klc_next_router); return KLC_OK;
+    case 4: *out_bytes = sizeof(klc_attn_dims); return KLC_OK;
     default: return klc::fail(KLC_ERR_INVALID, "klc_struct_size: unknown structure");
   }
 }
