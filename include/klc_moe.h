@@ -477,6 +477,95 @@ int klc_attn_prompt(const klc_attn_dims* dims, const void* q, int64_t q_tokens, 
                     const int32_t* cu_k, int64_t batch, const float* sinks, void* out, int64_t out_token_stride,
                     int64_t out_head_stride, float* lse, void* status, void* stream);
 
+/* Attention of one token per sequence over a paged cache: row b of q [batch,
+ * heads, D] sees the last `window` (or all) of the lens[b] keys that the pages
+ * block_table[b] = (table_width int32 page ids, rows table_stride apart) hold.
+ * A pool is [pages, kv_heads, page_size, D] with pages page_stride elements
+ * apart; page_size 16, 32, 64 or 128; keys and values have pools of their own.
+ * Everything a row does not see (past lens[b], before the window) may hold
+ * anything, and table entries of pages without a visible key are not read.
+ * Shared prefixes: `groups` > 0 groups of consecutive rows, group g the rows
+ * group_starts[g] .. group_starts[g+1] (int32 on the device, ascending), whose
+ * first prefix_lens[g] keys (a multiple of page_size) are the same pages: they
+ * are read once for the whole group, through the table of its first row; rows outside the groups have none.
+ * The split over SMs is made on the device from lens, so a captured call
+ * serves other lengths on replay.  Results do not depend on timing.  A page id
+ * outside [0, pages) and a length outside [0, table_width * page_size] are
+ * recorded as KLC_ERR_DEVICE_FAULT.  At most 4096 sequences.  One workspace
+ * per call in flight.  Replaces StreamedAttention.forward over the
+ * KVCacheManager's list (streamed_attention.py:100-152).                    */
+int klc_attn_decode_workspace_size(const klc_attn_dims* dims, int64_t batch, int64_t groups, size_t* out_bytes);
+int klc_attn_decode(const klc_attn_dims* dims, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                    const void* k_pages, const void* v_pages, int64_t pages, int page_size, int64_t page_stride,
+                    const int32_t* block_table, int64_t table_width, int64_t table_stride, const int32_t* lens,
+                    int64_t batch, const int32_t* group_starts, const int32_t* prefix_lens, int64_t groups,
+                    const float* sinks, void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                    void* workspace, size_t workspace_bytes, void* status, void* stream);
+
+/* Rotary embedding of new tokens and their write into the cache: q_out and the
+ * pages' keys get (x1 c - x2 s, x2 c + x1 s) of q and k, x1 and x2 the halves of
+ * a head's row, c and s the rows positions[t] of cos and sin (fp32 [max_pos,
+ * D / 2], contiguous), computed in fp32 and rounded once; the pages' values
+ * get v.  Token t goes to key positions[t] of the sequence block_table[rows[t]]
+ * (both int32 on the device; the pages must be there already: klc_kv_reserve).
+ * A token with rows[t] = -1 is padding: nothing is written for it.  q_out may
+ * be q; k_out (or NULL) receives the rotated keys as rows too.  Two tokens with
+ * the same row and position leave either's key and value.  Rows, positions and
+ * page ids out of range are recorded as KLC_ERR_DEVICE_FAULT and the token is
+ * skipped.  Strides and pools as for klc_attn_decode.  (apply_rope of
+ * streamed_attention.py, KVCacheManager's append kv_cache_manager.py:50-66) */
+int klc_rope_append(const klc_attn_dims* dims, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                    int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                    int64_t v_head_stride, const float* cos, const float* sin, int64_t max_pos, const int32_t* positions,
+                    const int32_t* rows, int64_t tokens, void* q_out, int64_t qo_token_stride, int64_t qo_head_stride,
+                    void* k_out, int64_t ko_token_stride, int64_t ko_head_stride, void* k_pages, void* v_pages,
+                    int64_t pages, int page_size, int64_t page_stride, const int32_t* block_table, int64_t table_rows,
+                    int64_t table_width, int64_t table_stride, void* status, void* stream);
+
+/* ---- pages of the key/value cache ----------------------------------------
+ * `planes` arrays of pages (keys and values of each layer), plane_stride bytes
+ * apart, page i at i * page_bytes; refs int32 [pages], reference counts, 0 for
+ * a free page; block_table int32 [rows][table_width], the page ids of each
+ * sequence; lens int32 [rows], its number of keys.  All on the device, all
+ * decisions too: no call synchronises, and every call can be captured.  New
+ * pages are the free ones with the lowest ids, given to the requests in list
+ * order.  A request that cannot be met (no pages left, a row that does not
+ * exist, a length past the table) is recorded in status as
+ * KLC_ERR_DEVICE_FAULT and leaves its row as it was; the others are served.
+ * Calls on one cache are ordered on one stream and share one workspace.     */
+typedef struct klc_kv_cache {
+  void* pool;
+  int64_t planes;
+  int64_t plane_stride; /* bytes, multiple of 16 */
+  int64_t page_bytes;   /* multiple of 16        */
+  int64_t pages;
+  int32_t* refs;        /* 16-byte aligned       */
+  int32_t* block_table;
+  int64_t table_width;
+  int64_t table_stride;
+  int32_t* lens;
+  int64_t rows;
+  int32_t page_size;    /* 16, 32, 64 or 128 keys */
+  void* status;         /* klc_status_bytes, or NULL */
+} klc_kv_cache;
+int klc_kv_workspace_size(const klc_kv_cache* cache, size_t* out_bytes);
+/* Every row r grows by add[r] >= 0 keys (int32 [rows]): the pages it needs are
+ * taken and lens advanced.  A row whose last page is shared cannot occur:
+ * klc_kv_fork copies a partial last page.                                   */
+int klc_kv_reserve(const klc_kv_cache* cache, const int32_t* add, void* workspace, size_t workspace_bytes, void* stream);
+/* Row children[i], which must be empty and listed once, becomes a copy of row
+ * parents[i]: the parent's full pages are shared and a partial last page is
+ * copied to a new one; with `copy` all pages are.  n <= rows.               */
+int klc_kv_fork(const klc_kv_cache* cache, const int32_t* parents, const int32_t* children, int64_t n, int copy,
+                void* workspace, size_t workspace_bytes, void* stream);
+/* The n listed rows become empty; pages nobody else refers to become free.  A
+ * row listed twice is freed once.                                           */
+int klc_kv_free(const klc_kv_cache* cache, const int32_t* rows, int64_t n, void* stream);
+/* The live pages with the highest ids move into the lowest free ones until the
+ * live pages are 0 .. n_live - 1; tables follow.  n_live int32 [1] on the
+ * device, or NULL.                                                          */
+int klc_kv_compact(const klc_kv_cache* cache, int32_t* n_live, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- expert parallelism over NVLink peer memory ------------------------
  * No counterpart in the reference (one process, one device): the node-level
  * sharding of the MoE block, rank r owning experts [r*epr, (r+1)*epr).  One

@@ -117,6 +117,24 @@ class KlcAttnDims(ctypes.Structure):
     ]
 
 
+class KlcKvCache(ctypes.Structure):
+    _fields_ = [
+        ("pool", c_void_p),
+        ("planes", c_int64),
+        ("plane_stride", c_int64),
+        ("page_bytes", c_int64),
+        ("pages", c_int64),
+        ("refs", c_void_p),
+        ("block_table", c_void_p),
+        ("table_width", c_int64),
+        ("table_stride", c_int64),
+        ("lens", c_void_p),
+        ("rows", c_int64),
+        ("page_size", c_int32),
+        ("status", c_void_p),
+    ]
+
+
 # name -> argtypes (every entry point returns int, except klc_last_error)
 SIGNATURES: dict[str, list] = {
     "klc_version": [],
@@ -186,6 +204,18 @@ SIGNATURES: dict[str, list] = {
     "klc_attn_prompt": [POINTER(KlcAttnDims), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
                         c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
                         c_void_p],
+    "klc_attn_decode_workspace_size": [POINTER(KlcAttnDims), c_int64, c_int64, POINTER(c_size_t)],
+    "klc_attn_decode": [POINTER(KlcAttnDims), c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int64, c_void_p,
+                        c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+                        c_void_p, c_void_p, c_size_t, c_void_p, c_void_p],
+    "klc_rope_append": [POINTER(KlcAttnDims), c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                        c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                        c_int64, c_void_p, c_void_p, c_int64, c_int, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p],
+    "klc_kv_workspace_size": [POINTER(KlcKvCache), POINTER(c_size_t)],
+    "klc_kv_reserve": [POINTER(KlcKvCache), c_void_p, c_void_p, c_size_t, c_void_p],
+    "klc_kv_fork": [POINTER(KlcKvCache), c_void_p, c_void_p, c_int64, c_int, c_void_p, c_size_t, c_void_p],
+    "klc_kv_free": [POINTER(KlcKvCache), c_void_p, c_int64, c_void_p],
+    "klc_kv_compact": [POINTER(KlcKvCache), c_void_p, c_void_p, c_size_t, c_void_p],
     "klc_rms_norm": [c_void_p, c_void_p, c_int64, c_int64, c_float, c_void_p, c_void_p],
     "klc_runtime_dequant": [c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int64, c_void_p, c_int, c_void_p],
 }
@@ -213,7 +243,7 @@ def lib() -> ctypes.CDLL:
     h.klc_last_error.argtypes = []
     h.klc_last_error.restype = c_char_p
     # the structures passed by pointer must have the library's layout
-    for which, struct in enumerate((KlcDims, KlcWeights, KlcLocalityConfig, KlcNextRouter, KlcAttnDims)):
+    for which, struct in enumerate((KlcDims, KlcWeights, KlcLocalityConfig, KlcNextRouter, KlcAttnDims, KlcKvCache)):
         n = c_size_t(0)
         if h.klc_struct_size(which, ctypes.byref(n)) != KLC_OK or n.value != ctypes.sizeof(struct):
             raise ImportError(f"{LIB_PATH} was built with another {struct.__name__} layout ({n.value} B) than this "

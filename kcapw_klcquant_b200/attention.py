@@ -4,7 +4,12 @@ The reference's :class:`StreamedAttention` (streamed_attention.py:100-152) runs
 one token at a time against a Python list of keys and values.  Here a batch of
 sequences is one call:
 
-* :func:`attn_prompt` -- causal attention over packed prompts of any lengths,
+* :func:`attn_prompt` -- causal attention over packed prompts of any lengths;
+* :func:`attn_decode` -- one new token per sequence over the paged cache
+  (:class:`~kcapw_klcquant_b200.kv_cache.PagedKvCache`), a prefix that a group
+  of sequences shares read once;
+* :func:`rope_append` -- rotary embedding of new tokens and their write into the
+  cache,
 
 with grouped heads, attention sinks and a sliding window as the reference has
 them.  Elements are bf16 or f16, head width 64 or 128; softmax statistics are
@@ -18,6 +23,7 @@ import threading
 import torch
 
 from . import _lib
+from .moe import workspace
 
 _STATUS: dict[int, torch.Tensor] = {}
 _STATUS_LOCK = threading.Lock()
@@ -176,3 +182,156 @@ def attn_prompt(
             k.shape[0], cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, _lib.ptr(sk), o.data_ptr(), *_strides(o),
             _lib.ptr(lse), _lib.ptr(device_status(dev)), _lib.stream_ptr(dev)))
     return (o, lse) if return_lse else o
+
+
+def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    """Scratch for one call: the stream's own, or, under capture, memory of the graph (two captured
+    graphs never share it, on whichever streams they are replayed)."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return workspace(device, nbytes, _lib.stream_ptr(device))
+
+
+def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype, device: torch.device, d: int) -> int:
+    """Checks a pair of page pools [pages, kv_heads, page_size, D] and returns their common page stride."""
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        check_tensor(name, t, dtype, device, 4)
+        if t.shape[3] != d:
+            raise ValueError(f"{name} must be [pages, kv_heads, page_size, {d}], got {tuple(t.shape)}")
+        if t.shape[1:].numel() and not t[:1].is_contiguous():
+            raise ValueError(f"{name}: a page must be contiguous")
+    if k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages and v_pages must have the same shape")
+    if k_pages.shape[0] < 1:
+        raise ValueError("the pools have no pages")
+    if k_pages.shape[0] == 1:
+        return k_pages.shape[1:].numel()
+    if k_pages.stride(0) != v_pages.stride(0):
+        raise ValueError("k_pages and v_pages must have the same page stride")
+    return k_pages.stride(0)
+
+
+def _table(block_table: torch.Tensor, device: torch.device) -> tuple[torch.Tensor, int]:
+    check_tensor("block_table", block_table, torch.int32, device, 2)
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        raise ValueError("block_table rows must be contiguous")
+    if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("block_table rows overlap")
+    return block_table, (block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1])
+
+
+def attn_decode(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    lens: torch.Tensor,
+    *,
+    scale: float | None = None,
+    window: int = 0,
+    sinks: torch.Tensor | None = None,
+    group_starts: torch.Tensor | None = None,
+    prefix_lens: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    return_lse: bool = False,
+):
+    """Attention of one token per sequence over its pages: q [B, heads, D].
+
+    ``k_pages`` and ``v_pages`` are pools [pages, kv_heads, page_size, D]
+    (page_size 16, 32, 64 or 128); row b sees the ``lens[b]`` keys of the pages
+    ``block_table[b]`` (int32 [B, width]), the own one among them, or the last
+    ``window`` of them.  ``sinks`` as for :func:`attn_prompt`.  With
+    ``group_starts`` (int32 [G + 1]) and ``prefix_lens`` (int32 [G], multiples of
+    page_size) the rows ``group_starts[g]:group_starts[g + 1]`` share the pages of
+    their first ``prefix_lens[g]`` keys, which are then read once for all of them,
+    through the first row's table.  At most 4096 rows.  Lengths stay on the device: a captured
+    call serves other lengths on replay.  Returns out [B, heads, D] (and the
+    log-sum-exp fp32 [B, heads] with ``return_lse``).
+    """
+    dev = _require_cuda(q)
+    if q.dim() != 3 or k_pages.dim() != 4:
+        raise ValueError("q must be [batch, heads, D] and the pools [pages, kv_heads, page_size, D]")
+    dims = _dims(q, int(k_pages.shape[1]), window, scale)
+    page_stride = _pools(k_pages, v_pages, q.dtype, dev, int(q.shape[2]))
+    B = int(q.shape[0])
+    table, table_stride = _table(block_table, dev)
+    ln = _offsets("lens", lens, dev)
+    if table.shape[0] != B or ln.numel() != B:
+        raise ValueError(f"block_table and lens must have {B} rows")
+    if (group_starts is None) != (prefix_lens is None):
+        raise ValueError("group_starts and prefix_lens go together")
+    gs = None if group_starts is None else _offsets("group_starts", group_starts, dev)
+    pl = None if prefix_lens is None else _offsets("prefix_lens", prefix_lens, dev)
+    groups = 0 if pl is None else pl.numel()
+    if gs is not None and gs.numel() != groups + 1:
+        raise ValueError("group_starts must have one element more than prefix_lens")
+    q = _rows("q", q, q.dtype, dev)
+    sk = _sinks(sinks, dims.heads, dev)
+    o = _out(out, q)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
+    with torch.cuda.device(dev):
+        n = ctypes.c_size_t(0)
+        _lib.check(_lib.lib().klc_attn_decode_workspace_size(ctypes.byref(dims), B, groups, ctypes.byref(n)))
+        ws = _workspace(dev, n.value)
+        _lib.check(_lib.lib().klc_attn_decode(
+            ctypes.byref(dims), q.data_ptr(), *_strides(q), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0],
+            int(k_pages.shape[2]), page_stride, table.data_ptr(), table.shape[1], table_stride, ln.data_ptr(), B, _lib.ptr(gs),
+            _lib.ptr(pl), groups, _lib.ptr(sk), o.data_ptr(), *_strides(o), _lib.ptr(lse), ws.data_ptr(), ws.numel(),
+            _lib.ptr(device_status(dev)), _lib.stream_ptr(dev)))
+    return (o, lse) if return_lse else o
+
+
+def rope_append(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    positions: torch.Tensor,
+    rows: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    *,
+    out: torch.Tensor | None = None,
+    return_k: bool = False,
+):
+    """Rotary embedding of q [T, heads, D] and k [T, kv_heads, D], and the write of k and v into the cache.
+
+    Token t is key ``positions[t]`` of sequence ``rows[t]`` (int32 on the device;
+    row -1: padding, nothing is written); its page must be reserved.  ``cos`` and
+    ``sin`` are fp32 [max_pos, D / 2]; the halves of a head's row are rotated
+    against each other, in fp32, rounded once.  Returns the rotated queries
+    (``out``, which may be q), and with ``return_k`` the rotated keys [T, kv_heads, D] too.
+    """
+    dev = _require_cuda(q)
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError("q, k and v must be [tokens, heads, D]")
+    T, d = int(q.shape[0]), int(q.shape[2])
+    dims = _dims(q, int(k.shape[1]), 0, 1.0)
+    if k.shape != v.shape or k.shape[0] != T or k.shape[2] != d:
+        raise ValueError(f"k and v must both be [{T}, kv_heads, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    page_stride = _pools(k_pages, v_pages, q.dtype, dev, d)
+    if k_pages.shape[1] != k.shape[1]:
+        raise ValueError(f"the pools have {k_pages.shape[1]} key heads, k has {k.shape[1]}")
+    for name, t in (("cos", cos), ("sin", sin)):
+        check_tensor(name, t, torch.float32, dev, 2)
+        if t.shape[1] != d // 2 or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous [max_pos, {d // 2}]")
+    if cos.shape != sin.shape:
+        raise ValueError("cos and sin must have the same shape")
+    table, table_stride = _table(block_table, dev)
+    pos, rw = _offsets("positions", positions, dev), _offsets("rows", rows, dev)
+    if pos.numel() != T or rw.numel() != T:
+        raise ValueError(f"positions and rows must have {T} elements")
+    q, k, v = _rows("q", q, q.dtype, dev), _rows("k", k, q.dtype, dev), _rows("v", v, q.dtype, dev)
+    o = _out(out, q)
+    ko = torch.empty(k.shape, dtype=k.dtype, device=dev) if return_k else None
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().klc_rope_append(
+            ctypes.byref(dims), q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), cos.data_ptr(),
+            sin.data_ptr(), cos.shape[0], pos.data_ptr(), rw.data_ptr(), T, o.data_ptr(), *_strides(o), _lib.ptr(ko),
+            *(_strides(ko) if ko is not None else (0, 0)), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0],
+            int(k_pages.shape[2]), page_stride, table.data_ptr(), table.shape[0], table.shape[1], table_stride,
+            _lib.ptr(device_status(dev)), _lib.stream_ptr(dev)))
+    return (o, ko) if return_k else o

@@ -153,6 +153,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   Item* item_s = reinterpret_cast<Item*>(smem + C::OFF_MISC + 8);
   const Ctl ctl{abort_flag, p.status};
 
+  if (PREFIX) pdl_trigger();  // the decode kernel may run beside this one
+
   // ---- which sequence (group) and rows: warp 0 walks the sequences' numbers of row-tile pairs
   if (warp == 0) {
     const int n_seq = p.batch;
@@ -552,6 +554,8 @@ int rows_map(CUtensorMap* m, int dtype, int head_dim, const void* base, int64_t 
   return make_map(m, map_type(dtype), 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+}  // namespace
+
 int check_rows(const char* who, const char* what, const void* base, int64_t tokens, int64_t ts, int64_t hs, int heads, int d) {
   const std::string w = std::string(who) + ": " + what;
   KLC_CHECK_ARG(base != nullptr, w + " is null");
@@ -562,14 +566,44 @@ int check_rows(const char* who, const char* what, const void* base, int64_t toke
   return KLC_OK;
 }
 
-}  // namespace
-
 int pool_map(CUtensorMap* m, int dtype, int head_dim, const void* base, int64_t pages, int kv_heads, int page_size,
              int64_t page_stride, int box_rows) {
   const uint64_t dims[4] = {uint64_t(head_dim), uint64_t(page_size), uint64_t(kv_heads), uint64_t(pages)};
   const uint64_t strides[3] = {uint64_t(head_dim) * 2, uint64_t(page_size) * head_dim * 2, uint64_t(page_stride) * 2};
   const uint32_t box[4] = {64, uint32_t(box_rows), 1, 1};
   return make_map(m, map_type(dtype), 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int launch_prefix(const klc_attn_dims& dims, const DecodeParams& d, const void* q, const void* k_pages, const void* v_pages,
+                  int64_t page_stride, cudaStream_t stream) {
+  TcParams p{};
+  p.cu_q = d.group_starts;
+  p.batch = d.groups;
+  p.total_q = d.batch;
+  p.total_k = int64_t(d.table_width) * d.page_size;
+  p.heads = d.heads;
+  p.group = d.group;
+  p.tpt = kRows / d.group;
+  p.scale_log2 = d.scale_log2;
+  p.window = d.window;
+  p.status = d.status;
+  p.prefix_lens = d.prefix_lens;
+  p.lens = d.lens;
+  p.block_table = d.block_table;
+  p.table_stride = d.table_stride;
+  p.pages = d.pages;
+  p.page_size = d.page_size;
+  p.part_o = d.prefix_o;
+  p.part_ml = d.prefix_ml;
+  CUtensorMap mq, mk, mv;
+  int st = rows_map(&mq, dims.dtype, dims.head_dim, q, d.batch, d.heads, d.q_ts, d.q_hs, d.group, p.tpt);
+  if (st == KLC_OK) st = pool_map(&mk, dims.dtype, dims.head_dim, k_pages, d.pages, d.kv_heads, d.page_size, page_stride, d.page_size);
+  if (st == KLC_OK) st = pool_map(&mv, dims.dtype, dims.head_dim, v_pages, d.pages, d.kv_heads, d.page_size, page_stride, d.page_size);
+  if (st != KLC_OK) return st;
+  const int tok = 2 * p.tpt;
+  const int pairs = d.groups == 1 ? (d.batch + tok - 1) / tok : std::min(d.batch, d.batch / tok + d.groups);
+  return launch_typed<true>(dims.dtype, dims.head_dim, mq, mk, mv, p,
+                            dim3(unsigned(pairs), unsigned(d.kv_heads), unsigned(d.splits)), stream);
 }
 
 }  // namespace attn

@@ -110,6 +110,7 @@ extern "C" int klc_struct_size(int which, size_t* out_bytes) {
     case 2: *out_bytes = sizeof(klc_locality_config); return KLC_OK;
     case 3: *out_bytes = sizeof(klc_next_router); return KLC_OK;
     case 4: *out_bytes = sizeof(klc_attn_dims); return KLC_OK;
+    case 5: *out_bytes = sizeof(klc_kv_cache); return KLC_OK;
     default: return klc::fail(KLC_ERR_INVALID, "klc_struct_size: unknown structure");
   }
 }
