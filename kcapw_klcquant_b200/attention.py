@@ -29,20 +29,19 @@ _STATUS: dict[int, torch.Tensor] = {}
 _STATUS_LOCK = threading.Lock()
 
 
-def device_status(device: torch.device) -> torch.Tensor | None:
-    """The device's fault word (klc_status_bytes, zeroed once).  None while a graph is being
+def device_status(index: int) -> torch.Tensor | None:
+    """The fault word of CUDA device ``index`` (klc_status_bytes, zeroed once).  None while a graph is being
     captured before the first eager call made it: that graph then records no faults."""
-    idx = device.index
-    st = _STATUS.get(idx)
+    st = _STATUS.get(index)
     if st is None and not torch.cuda.is_current_stream_capturing():
         with _STATUS_LOCK:
-            st = _STATUS.get(idx)
+            st = _STATUS.get(index)
             if st is None:
                 n = ctypes.c_size_t(0)
                 _lib.check(_lib.lib().klc_status_bytes(ctypes.byref(n)))
-                st = torch.zeros(n.value, dtype=torch.uint8, device=device)
-                torch.cuda.current_stream(device).synchronize()  # zeroed before a call on any other stream
-                _STATUS[idx] = st
+                st = torch.zeros(n.value, dtype=torch.uint8, device=torch.device("cuda", index))
+                torch.cuda.current_stream(index).synchronize()  # zeroed before a call on any other stream
+                _STATUS[index] = st
     return st
 
 
@@ -54,86 +53,103 @@ def check_device_status(device: torch.device | str | int = "cuda") -> None:
     other streams are seen by a later check.
     """
     dev = torch.device(device)
-    if dev.index is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
-    st = _STATUS.get(dev.index)
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    st = _STATUS.get(index)
     if st is None:
         return
-    with torch.cuda.device(dev):
+    with on_device(index) as stream:
         try:
-            _lib.check(_lib.lib().klc_workspace_status(st.data_ptr(), None, None, None, _lib.stream_ptr(dev)))
+            _lib.check(_lib.lib().klc_workspace_status(st.data_ptr(), None, None, None, stream))
         except _lib.KlcError:
             st.zero_()
             raise
 
 
-def check_tensor(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, ndim: int) -> None:
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != ndim:
-        raise ValueError(f"{name} must have {ndim} dimensions, got {tuple(t.shape)}")
+def check_tensor(name: str, t: torch.Tensor, dtype: torch.dtype, index: int, ndim: int) -> None:
+    """``t`` has the dtype and number of dimensions and is on CUDA device ``index``."""
+    if t.get_device() != index or t.dtype is not dtype or t.dim() != ndim:
+        raise ValueError(f"{name} must be {dtype} with {ndim} dimensions on cuda:{index}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """A [tokens, heads, D] operand the kernels can address: contiguous rows, 16-byte aligned strides."""
-    check_tensor(name, t, dtype, device, 3)
-    if t.numel() == 0:
-        return t
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0
-    for dim in (0, 1):
-        if t.shape[dim] > 1:
-            ok = ok and t.stride(dim) % 8 == 0 and t.stride(dim) >= t.shape[2]
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, index: int) -> tuple[torch.Tensor, int, int, int]:
+    """A [tokens, heads, D] operand as the kernels address it: (tensor, address, token stride, head stride).
+
+    Rows are contiguous and 16-byte aligned, strides multiples of 8 elements; anything else is copied.  A
+    dimension of one row gets a contiguous stride.
+    """
+    check_tensor(name, t, dtype, index, 3)
+    n, h, d = t.shape
+    ts, hs, one = t.stride()
+    if h == 1:
+        hs = d
+    if n == 1:
+        ts = h * max(hs, d)
+    ptr = t.data_ptr()
+    if (one != 1 or ptr & 15 or ts & 7 or hs & 7 or ts < d or hs < d) and t.numel():
+        t = t.clone(memory_format=torch.contiguous_format)
+        return t, t.data_ptr(), h * d, d
+    return t, ptr, ts, hs
 
 
-def _strides(t: torch.Tensor) -> tuple[int, int]:
-    """Token and head strides in elements; a dimension of one row gets the contiguous stride."""
-    d = t.shape[2]
-    hs = t.stride(1) if t.shape[1] > 1 else d
-    ts = t.stride(0) if t.shape[0] > 1 else t.shape[1] * max(hs, d)
-    return ts, hs
+def _ints(name: str, t: torch.Tensor, index: int) -> torch.Tensor:
+    check_tensor(name, t, torch.int32, index, 1)
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _offsets(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
-    check_tensor(name, t, torch.int32, device, 1)
-    return t.contiguous()
-
-
-def _sinks(sinks: torch.Tensor | None, heads: int, device: torch.device) -> torch.Tensor | None:
+def _sinks(sinks: torch.Tensor | None, heads: int, index: int) -> torch.Tensor | None:
     if sinks is None:
         return None
-    check_tensor("sinks", sinks, torch.float32, device, 1)
-    if sinks.numel() != heads:
+    check_tensor("sinks", sinks, torch.float32, index, 1)
+    if sinks.shape[0] != heads:
         raise ValueError(f"sinks must have {heads} elements")
-    return sinks.contiguous()
+    return sinks if sinks.is_contiguous() else sinks.contiguous()
 
 
 def _dims(q: torch.Tensor, kv_heads: int, window: int, scale: float | None) -> _lib.KlcAttnDims:
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    code = _lib.DTYPE_CODE.get(q.dtype)
+    if code is None or q.dtype is torch.float32:
         raise ValueError(f"attention expects bf16 or f16, got {q.dtype}")
-    heads, d = int(q.shape[1]), int(q.shape[2])
-    if not 0 <= int(window) < 1 << 31:
+    if not 0 <= window < 1 << 31:
         raise ValueError("window must be >= 0 and fit 32 bits")
-    return _lib.KlcAttnDims(_lib.DTYPE_CODE[q.dtype], heads, kv_heads, d, int(window), float(d ** -0.5 if scale is None else scale))
+    _, heads, d = q.shape
+    return _lib.KlcAttnDims(code, heads, kv_heads, d, window, d ** -0.5 if scale is None else scale)
 
 
-def _out(out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
+def _out(out: torch.Tensor | None, q: torch.Tensor, index: int) -> tuple[torch.Tensor, int, int, int]:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    check_tensor("out", out, q.dtype, q.device, 3)
-    if out.shape != q.shape:
+        out = q.new_empty(q.shape)
+    elif out.shape != q.shape:
         raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
-    if out.numel() and _rows("out", out, q.dtype, q.device) is not out:
+    got = _rows("out", out, q.dtype, index)
+    if got[0] is not out:
         raise ValueError("out must have contiguous, 16-byte aligned rows and strides of multiples of 8 elements")
-    return out
+    return got
 
 
-def _require_cuda(t: torch.Tensor) -> torch.device:
-    if not t.is_cuda:
+def _device_of(q: torch.Tensor) -> int:
+    if not q.is_cuda:
         raise ValueError("kcapw_klcquant_b200 runs on CUDA devices only (no CPU fallback); got a CPU tensor")
-    return t.device
+    return q.get_device()
+
+
+class on_device:
+    """``torch.cuda.device`` that costs nothing when the device is current already; gives the current stream."""
+
+    __slots__ = ("index", "guard")
+
+    def __init__(self, index: int):
+        self.index = index
+        self.guard = None
+
+    def __enter__(self) -> int:
+        if torch.cuda.current_device() != self.index:
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+        return _lib.stream_ptr(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def attn_prompt(
@@ -160,64 +176,71 @@ def attn_prompt(
     ``out`` past the last sequence are not written.  Returns out [T, heads, D]
     (and the log-sum-exp fp32 [T, heads] with ``return_lse``).
     """
-    dev = _require_cuda(q)
+    dev = _device_of(q)
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q, k and v must be [tokens, heads, D]")
-    dims = _dims(q, int(k.shape[1]), window, scale)
-    if k.shape != v.shape or k.shape[2] != q.shape[2]:
-        raise ValueError(f"k and v must both be [tokens, kv_heads, {q.shape[2]}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    cu_q = _offsets("cu_seqlens", cu_seqlens, dev)
-    cu_k = cu_q if cu_seqlens_k is None else _offsets("cu_seqlens_k", cu_seqlens_k, dev)
-    if cu_q.numel() < 1 or cu_q.numel() != cu_k.numel():
+    T, _, d = q.shape
+    Tk, kv_heads, dk = k.shape
+    dims = _dims(q, kv_heads, window, scale)
+    if k.shape != v.shape or dk != d:
+        raise ValueError(f"k and v must both be [tokens, kv_heads, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    cu_q = _ints("cu_seqlens", cu_seqlens, dev)
+    cu_k = cu_q if cu_seqlens_k is None else _ints("cu_seqlens_k", cu_seqlens_k, dev)
+    batch = cu_q.shape[0] - 1
+    if batch < 0 or cu_k.shape[0] != batch + 1:
         raise ValueError("cu_seqlens (and cu_seqlens_k) must have batch + 1 elements")
-    if cu_seqlens_k is None and k.shape[0] != q.shape[0]:
+    if cu_seqlens_k is None and Tk != T:
         raise ValueError("q and k have different numbers of rows: give cu_seqlens_k")
-    q, k, v = _rows("q", q, q.dtype, dev), _rows("k", k, q.dtype, dev), _rows("v", v, q.dtype, dev)
+    q, *qa = _rows("q", q, q.dtype, dev)
+    k, *ka = _rows("k", k, q.dtype, dev)
+    v, *va = _rows("v", v, q.dtype, dev)
     sk = _sinks(sinks, dims.heads, dev)
-    o = _out(out, q)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
-    with torch.cuda.device(dev):
+    o, *oa = _out(out, q, dev)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    with on_device(dev) as stream:
         _lib.check(_lib.lib().klc_attn_prompt(
-            ctypes.byref(dims), q.data_ptr(), q.shape[0], *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v),
-            k.shape[0], cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, _lib.ptr(sk), o.data_ptr(), *_strides(o),
-            _lib.ptr(lse), _lib.ptr(device_status(dev)), _lib.stream_ptr(dev)))
+            ctypes.byref(dims), qa[0], T, qa[1], qa[2], *ka, *va, Tk, cu_q.data_ptr(), cu_k.data_ptr(), batch, _lib.ptr(sk), *oa,
+            _lib.ptr(lse), _lib.ptr(device_status(dev)), stream))
     return (o, lse) if return_lse else o
 
 
-def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+def _workspace(device: torch.device, nbytes: int, stream: int) -> torch.Tensor:
     """Scratch for one call: the stream's own, or, under capture, memory of the graph (two captured
     graphs never share it, on whichever streams they are replayed)."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return workspace(device, nbytes, _lib.stream_ptr(device))
+    return workspace(device, nbytes, stream)
 
 
-def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype, device: torch.device, d: int) -> int:
-    """Checks a pair of page pools [pages, kv_heads, page_size, D] and returns their common page stride."""
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        check_tensor(name, t, dtype, device, 4)
-        if t.shape[3] != d:
-            raise ValueError(f"{name} must be [pages, kv_heads, page_size, {d}], got {tuple(t.shape)}")
-        if t.shape[1:].numel() and not t[:1].is_contiguous():
-            raise ValueError(f"{name}: a page must be contiguous")
-    if k_pages.shape != v_pages.shape:
-        raise ValueError("k_pages and v_pages must have the same shape")
-    if k_pages.shape[0] < 1:
-        raise ValueError("the pools have no pages")
-    if k_pages.shape[0] == 1:
-        return k_pages.shape[1:].numel()
-    if k_pages.stride(0) != v_pages.stride(0):
+def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype, index: int, d: int) -> tuple[int, int]:
+    """Checks a pair of page pools [pages, kv_heads, page_size, D]; (page size, common page stride)."""
+    check_tensor("k_pages", k_pages, dtype, index, 4)
+    check_tensor("v_pages", v_pages, dtype, index, 4)
+    shape, stride = k_pages.shape, k_pages.stride()
+    pages, heads, ps, width = shape
+    if v_pages.shape != shape or width != d or pages < 1:
+        raise ValueError(f"k_pages and v_pages must both be [pages, kv_heads, page_size, {d}], got {tuple(shape)} and {tuple(v_pages.shape)}")
+    want = (ps * d, d, 1)
+    if (stride[1:] != want or v_pages.stride()[1:] != want) and not (k_pages[0].is_contiguous() and v_pages[0].is_contiguous()):
+        raise ValueError("k_pages and v_pages: a page must be contiguous")
+    if pages == 1:
+        return ps, heads * ps * d
+    if stride[0] != v_pages.stride(0):
         raise ValueError("k_pages and v_pages must have the same page stride")
-    return k_pages.stride(0)
+    return ps, stride[0]
 
 
-def _table(block_table: torch.Tensor, device: torch.device) -> tuple[torch.Tensor, int]:
-    check_tensor("block_table", block_table, torch.int32, device, 2)
-    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+def _table(block_table: torch.Tensor, index: int) -> tuple[int, int, int]:
+    """Checks a page table; (rows, width, row stride)."""
+    check_tensor("block_table", block_table, torch.int32, index, 2)
+    (rows, width), (stride, one) = block_table.shape, block_table.stride()
+    if one != 1 and width > 1:
         raise ValueError("block_table rows must be contiguous")
-    if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
+    if rows <= 1:
+        stride = width
+    if stride < width:
         raise ValueError("block_table rows overlap")
-    return block_table, (block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1])
+    return rows, width, stride
 
 
 def attn_decode(
@@ -248,36 +271,39 @@ def attn_decode(
     call serves other lengths on replay.  Returns out [B, heads, D] (and the
     log-sum-exp fp32 [B, heads] with ``return_lse``).
     """
-    dev = _require_cuda(q)
+    dev = _device_of(q)
     if q.dim() != 3 or k_pages.dim() != 4:
         raise ValueError("q must be [batch, heads, D] and the pools [pages, kv_heads, page_size, D]")
-    dims = _dims(q, int(k_pages.shape[1]), window, scale)
-    page_stride = _pools(k_pages, v_pages, q.dtype, dev, int(q.shape[2]))
-    B = int(q.shape[0])
-    table, table_stride = _table(block_table, dev)
-    ln = _offsets("lens", lens, dev)
-    if table.shape[0] != B or ln.numel() != B:
+    B, _, d = q.shape
+    pages, kv_heads = k_pages.shape[:2]
+    dims = _dims(q, kv_heads, window, scale)
+    ps, page_stride = _pools(k_pages, v_pages, q.dtype, dev, d)
+    rows, width, table_stride = _table(block_table, dev)
+    ln = _ints("lens", lens, dev)
+    if rows != B or ln.shape[0] != B:
         raise ValueError(f"block_table and lens must have {B} rows")
-    if (group_starts is None) != (prefix_lens is None):
-        raise ValueError("group_starts and prefix_lens go together")
-    gs = None if group_starts is None else _offsets("group_starts", group_starts, dev)
-    pl = None if prefix_lens is None else _offsets("prefix_lens", prefix_lens, dev)
-    groups = 0 if pl is None else pl.numel()
-    if gs is not None and gs.numel() != groups + 1:
-        raise ValueError("group_starts must have one element more than prefix_lens")
-    q = _rows("q", q, q.dtype, dev)
+    gs = pl = None
+    groups = 0
+    if group_starts is not None or prefix_lens is not None:
+        if group_starts is None or prefix_lens is None:
+            raise ValueError("group_starts and prefix_lens go together")
+        gs, pl = _ints("group_starts", group_starts, dev), _ints("prefix_lens", prefix_lens, dev)
+        groups = pl.shape[0]
+        if gs.shape[0] != groups + 1:
+            raise ValueError("group_starts must have one element more than prefix_lens")
+    q, *qa = _rows("q", q, q.dtype, dev)
     sk = _sinks(sinks, dims.heads, dev)
-    o = _out(out, q)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
-    with torch.cuda.device(dev):
+    o, *oa = _out(out, q, dev)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    L = _lib.lib()
+    with on_device(dev) as stream:
         n = ctypes.c_size_t(0)
-        _lib.check(_lib.lib().klc_attn_decode_workspace_size(ctypes.byref(dims), B, groups, ctypes.byref(n)))
-        ws = _workspace(dev, n.value)
-        _lib.check(_lib.lib().klc_attn_decode(
-            ctypes.byref(dims), q.data_ptr(), *_strides(q), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0],
-            int(k_pages.shape[2]), page_stride, table.data_ptr(), table.shape[1], table_stride, ln.data_ptr(), B, _lib.ptr(gs),
-            _lib.ptr(pl), groups, _lib.ptr(sk), o.data_ptr(), *_strides(o), _lib.ptr(lse), ws.data_ptr(), ws.numel(),
-            _lib.ptr(device_status(dev)), _lib.stream_ptr(dev)))
+        _lib.check(L.klc_attn_decode_workspace_size(ctypes.byref(dims), B, groups, ctypes.byref(n)))
+        ws = _workspace(q.device, n.value, stream)
+        _lib.check(L.klc_attn_decode(
+            ctypes.byref(dims), *qa, k_pages.data_ptr(), v_pages.data_ptr(), pages, ps, page_stride, block_table.data_ptr(), width,
+            table_stride, ln.data_ptr(), B, _lib.ptr(gs), _lib.ptr(pl), groups, _lib.ptr(sk), *oa, _lib.ptr(lse), ws.data_ptr(),
+            ws.numel(), _lib.ptr(device_status(dev)), stream))
     return (o, lse) if return_lse else o
 
 
@@ -304,34 +330,37 @@ def rope_append(
     against each other, in fp32, rounded once.  Returns the rotated queries
     (``out``, which may be q), and with ``return_k`` the rotated keys [T, kv_heads, D] too.
     """
-    dev = _require_cuda(q)
+    dev = _device_of(q)
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q, k and v must be [tokens, heads, D]")
-    T, d = int(q.shape[0]), int(q.shape[2])
-    dims = _dims(q, int(k.shape[1]), 0, 1.0)
+    T, _, d = q.shape
+    kv_heads = k.shape[1]
+    dims = _dims(q, kv_heads, 0, 1.0)
     if k.shape != v.shape or k.shape[0] != T or k.shape[2] != d:
         raise ValueError(f"k and v must both be [{T}, kv_heads, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    page_stride = _pools(k_pages, v_pages, q.dtype, dev, d)
-    if k_pages.shape[1] != k.shape[1]:
-        raise ValueError(f"the pools have {k_pages.shape[1]} key heads, k has {k.shape[1]}")
-    for name, t in (("cos", cos), ("sin", sin)):
-        check_tensor(name, t, torch.float32, dev, 2)
-        if t.shape[1] != d // 2 or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous [max_pos, {d // 2}]")
-    if cos.shape != sin.shape:
-        raise ValueError("cos and sin must have the same shape")
-    table, table_stride = _table(block_table, dev)
-    pos, rw = _offsets("positions", positions, dev), _offsets("rows", rows, dev)
-    if pos.numel() != T or rw.numel() != T:
+    ps, page_stride = _pools(k_pages, v_pages, q.dtype, dev, d)
+    if k_pages.shape[1] != kv_heads:
+        raise ValueError(f"the pools have {k_pages.shape[1]} key heads, k has {kv_heads}")
+    check_tensor("cos", cos, torch.float32, dev, 2)
+    check_tensor("sin", sin, torch.float32, dev, 2)
+    max_pos, half = cos.shape
+    if cos.shape != sin.shape or 2 * half != d or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError(f"cos and sin must both be contiguous [max_pos, {d // 2}], got {tuple(cos.shape)} and {tuple(sin.shape)}")
+    rows_n, width, table_stride = _table(block_table, dev)
+    pos, rw = _ints("positions", positions, dev), _ints("rows", rows, dev)
+    if pos.shape[0] != T or rw.shape[0] != T:
         raise ValueError(f"positions and rows must have {T} elements")
-    q, k, v = _rows("q", q, q.dtype, dev), _rows("k", k, q.dtype, dev), _rows("v", v, q.dtype, dev)
-    o = _out(out, q)
-    ko = torch.empty(k.shape, dtype=k.dtype, device=dev) if return_k else None
-    with torch.cuda.device(dev):
+    q, *qa = _rows("q", q, q.dtype, dev)
+    k, *ka = _rows("k", k, q.dtype, dev)
+    v, *va = _rows("v", v, q.dtype, dev)
+    o, *oa = _out(out, q, dev)
+    ko, koa = None, (None, 0, 0)
+    if return_k:
+        ko = k.new_empty(k.shape)
+        koa = _rows("k_out", ko, q.dtype, dev)[1:]
+    with on_device(dev) as stream:
         _lib.check(_lib.lib().klc_rope_append(
-            ctypes.byref(dims), q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), cos.data_ptr(),
-            sin.data_ptr(), cos.shape[0], pos.data_ptr(), rw.data_ptr(), T, o.data_ptr(), *_strides(o), _lib.ptr(ko),
-            *(_strides(ko) if ko is not None else (0, 0)), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0],
-            int(k_pages.shape[2]), page_stride, table.data_ptr(), table.shape[0], table.shape[1], table_stride,
-            _lib.ptr(device_status(dev)), _lib.stream_ptr(dev)))
+            ctypes.byref(dims), *qa, *ka, *va, cos.data_ptr(), sin.data_ptr(), max_pos, pos.data_ptr(), rw.data_ptr(), T, *oa, *koa,
+            k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], ps, page_stride, block_table.data_ptr(), rows_n, width,
+            table_stride, _lib.ptr(device_status(dev)), stream))
     return (o, ko) if return_k else o

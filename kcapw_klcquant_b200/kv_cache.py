@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .attention import check_device_status, check_tensor, device_status
+from .attention import check_device_status, check_tensor, device_status, on_device
 
 
 class PagedKvCache:
@@ -50,7 +50,7 @@ class PagedKvCache:
         self._c = _lib.KlcKvCache(
             self.pool.data_ptr(), 2 * layers, self.pool.stride(1) * self.pool.element_size(),
             self.pool.stride(2) * self.pool.element_size(), pages, self.refs.data_ptr(), self.block_table.data_ptr(), row_pages,
-            row_pages, self.lens.data_ptr(), rows, page_size, _lib.ptr(device_status(dev)))
+            row_pages, self.lens.data_ptr(), rows, page_size, _lib.ptr(device_status(dev.index)))
         n = ctypes.c_size_t(0)
         _lib.check(_lib.lib().klc_kv_workspace_size(ctypes.byref(self._c), ctypes.byref(n)))
         self._ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
@@ -67,12 +67,12 @@ class PagedKvCache:
         return self.pool[layer, 1]
 
     def _list(self, name: str, t: torch.Tensor) -> torch.Tensor:
-        check_tensor(name, t, torch.int32, self.device, 1)
-        return t.contiguous()
+        check_tensor(name, t, torch.int32, self.device.index, 1)
+        return t if t.is_contiguous() else t.contiguous()
 
     def _call(self, fn, *args) -> None:
-        with torch.cuda.device(self.device):
-            _lib.check(fn(ctypes.byref(self._c), *args, _lib.stream_ptr(self.device)))
+        with on_device(self.device.index) as stream:
+            _lib.check(fn(ctypes.byref(self._c), *args, stream))
 
     def reserve(self, add: torch.Tensor) -> None:
         """Every row grows by ``add[row]`` keys: takes the pages it needs and advances ``lens``."""
