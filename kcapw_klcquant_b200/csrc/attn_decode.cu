@@ -446,37 +446,58 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const Decode
   }
   if (!prefix && first == last) return;  // written by the decode kernel
 
-  // shares: the prefix's splits, then the row's own keys: one share if uncut, else one per CTA
-  const int skip = prefix ? 0 : p.splits, own = last - first + 1, n = p.splits + own;
-  auto share = [&](int i) -> int64_t {  // row index into the prefix arrays, or (negative) ~row into the CTAs' shares
-    if (i < p.splits || own == 1) return (int64_t(i) * p.batch + b) * p.heads + head;
-    const int c = first + i - p.splits;
-    return ~(int64_t(2 * c + (total * c / nc < i0 ? 1 : 0)) * kRowTile + rr);
+  // Shares: the prefix's splits, then the row's own keys (one share if uncut, else one per CTA: the first CTA's second
+  // slot if the item starts inside its range, the first slot of the others).  Lane i holds share i's (m, l).
+  const int skip = prefix ? 0 : p.splits, own = last - first + 1, n = p.splits + own - skip;
+  const int64_t pre_row = int64_t(b) * p.heads + head, pre_step = int64_t(p.batch) * p.heads;
+  const bool inside = own > 1 && total * first / nc < i0;
+  auto share = [&](int i) -> int64_t {  // row index into the prefix arrays, or ~(row index) into the CTAs' shares
+    i += skip;
+    if (i < p.splits || own == 1) return pre_row + i * pre_step;
+    const int c = i - p.splits;
+    return ~(int64_t(2 * (first + c) + (c == 0 && inside ? 1 : 0)) * kRowTile + rr);
   };
-  auto share_ml = [&](int i) {
-    const int64_t r = share(i);
-    return r >= 0 ? p.prefix_ml[r] : p.part_ml[~r];
-  };
-  auto share_o = [&](int i) -> const float* {
-    const int64_t r = share(i);
-    return (r >= 0 ? p.prefix_o + r * D : p.part_o + ~r * D) + lane * V;
-  };
-  float top = -INFINITY;
-  for (int i = skip + lane; i < n; i += 32) top = fmaxf(top, share_ml(i).x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float sum = 0.f, acc[V];
+  float top = -INFINITY, sum = 0.f, acc[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
-#pragma unroll 4
-  for (int i = skip; i < n; ++i) {
-    const float2 a = share_ml(i);
-    if (a.x == -INFINITY) continue;  // a share without keys: its output was not written
-    const float f = exp2_approx(a.x - top);
-    sum += a.y * f;
-    const float* src = share_o(i);
+  for (int i0s = 0; i0s < n; i0s += 32) {
+    const int mine = i0s + lane;
+    int64_t at = 0;
+    float2 a = make_float2(-INFINITY, 0.f);
+    if (mine < n) {
+      at = share(mine);
+      a = at >= 0 ? p.prefix_ml[at] : p.part_ml[~at];
+    }
+    const float was = top;
+    float mx = a.x;
 #pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] += src[j] * f;
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    top = fmaxf(top, mx);
+    const float f = a.x == -INFINITY ? 0.f : exp2_approx(a.x - top);  // 0: no keys, and its output was not written
+    float part = warp_sum(a.y * f);
+    const float back = was == -INFINITY ? 0.f : exp2_approx(was - top);
+    sum = sum * back + part;
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] *= back;
+    const int count = min(32, n - i0s);
+#pragma unroll 8
+    for (int i = 0; i < count; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      const int64_t r = __shfl_sync(0xffffffffu, at, i);
+      if (fi == 0.f) continue;
+      const float* src = (r >= 0 ? p.prefix_o + r * D : p.part_o + ~r * D) + lane * V;
+      if constexpr (V == 2) {
+        const float2 x = *reinterpret_cast<const float2*>(src);
+        acc[0] += x.x * fi;
+        acc[1] += x.y * fi;
+      } else {
+        const float4 x = *reinterpret_cast<const float4*>(src);
+        acc[0] += x.x * fi;
+        acc[1] += x.y * fi;
+        acc[2] += x.z * fi;
+        acc[3] += x.w * fi;
+      }
+    }
   }
   float inv, lse;
   finish_row(top, sum, p.sinks != nullptr, p.sinks != nullptr ? p.sinks[head] * kLog2e : 0.f, &inv, &lse);

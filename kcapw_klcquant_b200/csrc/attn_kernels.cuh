@@ -14,7 +14,7 @@ struct TcParams {
   const int32_t* cu_k;  // prompts: [batch + 1] first key row
   int batch;
   int64_t total_q, total_k;
-  int heads, group, tpt;  // query heads; per key head; tokens per row tile
+  int heads, kv_heads, group, tpt;  // query and key heads; query heads per key head; tokens per row tile
   float scale_log2;       // scale * log2(e)
   int window;
   const float* sinks;
@@ -28,6 +28,7 @@ struct TcParams {
   const int32_t* block_table;
   int64_t table_stride, pages;
   int page_size;
+  int splits;       // shares the prefix's keys are cut into
   float* part_o;    // [splits][total_q][heads][D]
   float2* part_ml;  // [splits][total_q][heads]
 };

@@ -21,6 +21,7 @@
 // 2^8, far inside both types' range, and its relative rounding (2^-9 / 2^-12,
 // the price of a 16-bit P operand) does not depend on the reference maximum.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_common.cuh"
 #include "attn_kernels.cuh"
@@ -39,6 +40,7 @@ constexpr int kThreads = 320;  // 8 softmax warps, MMA warp, TMA warp
 constexpr int kWarpMma = 8, kWarpTma = 9;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;
+constexpr int kItems = 2;      // ring of items between the TMA warp and the others
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -75,6 +77,86 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16f(uint32_t taddr, float* v) {
+  uint32_t r[16];
+  tmem_ld16(taddr, r);
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
+}
+
+// waits for the loads into v; the operands keep their uses behind the wait
+__device__ __forceinline__ void tmem_wait_ld64(float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]), "+r"(r[32]), "+r"(r[33]), "+r"(r[34]), "+r"(r[35]), "+r"(r[36]), "+r"(r[37]), "+r"(r[38]), "+r"(r[39]), "+r"(r[40]), "+r"(r[41]), "+r"(r[42]), "+r"(r[43]), "+r"(r[44]), "+r"(r[45]), "+r"(r[46]), "+r"(r[47]), "+r"(r[48]), "+r"(r[49]), "+r"(r[50]), "+r"(r[51]), "+r"(r[52]), "+r"(r[53]), "+r"(r[54]), "+r"(r[55]), "+r"(r[56]), "+r"(r[57]), "+r"(r[58]), "+r"(r[59]), "+r"(r[60]), "+r"(r[61]), "+r"(r[62]), "+r"(r[63])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// pairs of fp32 in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// 2^x on the FMA pipe, for the share of a tile's exponentials that the special-function unit (16 a clock
+// and SM) would be late with: x = n + f, n the nearest integer (rounded by adding 1.5 * 2^23), 2^f a
+// polynomial fitted on [-1/2, 1/2] (relative error 7.5e-5, degree 3, beside bf16's 2^-9; 2.6e-6,
+// degree 4, beside f16's 2^-12), n added to the exponent.  x below -126 counts as -126.
+template <typename T>
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  const float2 big = make_float2(12582912.f, 12582912.f);
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 t = add2(x, big);
+  const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = add2(x, make_float2(-n.x, -n.y));
+  float2 p;
+  if constexpr (Elem<T>::kMmaFormat == 1) {
+    p = fma2(f, make_float2(0.05517166802f, 0.05517166802f), make_float2(0.24261112211f, 0.24261112211f));
+    p = fma2(f, p, make_float2(0.69326098565f, 0.69326098565f));
+    p = fma2(f, p, make_float2(0.99992807355f, 0.99992807355f));
+  } else {
+    p = fma2(f, make_float2(0.00957010179f, 0.00957010179f), make_float2(0.05591786031f, 0.05591786031f));
+    p = fma2(f, p, make_float2(0.24024744831f, 0.24024744831f));
+    p = fma2(f, p, make_float2(0.69312181474f, 0.69312181474f));
+    p = fma2(f, p, make_float2(0.99999926144f, 0.99999926144f));
+  }
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
 // D[tmem] (+)= A[tmem or smem] * B[smem]
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -105,29 +187,37 @@ __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t mn_st
          (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 
+struct Item {
+  int q0, qn;  // the sequence's first query row and its number of query rows (tokens)
+  int k0, kn;  // first key row and number of keys
+  int tok0;    // first token of the item's row tiles; -1: no more items
+  int tiles;   // row tiles with rows: 1 or 2
+  int lo, n;   // key tiles lo .. lo + n
+  int kvh, z;  // key head; prefix: share of the keys
+};
+
 template <int D>
 struct Cfg {
   static constexpr int kChunks = D / 64;                    // 128-byte columns of a head's row
   static constexpr int kTile = kKeys * D * 2;               // bytes of a query, key or value tile
   static constexpr int kStages = D == 64 ? 10 : 5;          // ring of key and value tiles: 160 KB
+  static constexpr int kFmaPairs = D == 64 ? 3 : 2;         // of 8 pairs of exponentials, on the FMA pipe
   static constexpr int OFF_Q = 0;                           // two row tiles
   static constexpr int OFF_KV = 2 * kTile;
   static constexpr int OFF_BAR = OFF_KV + kStages * kTile;
-  static constexpr int kBars = 1 + 2 * kStages + 2 + 2 + 2 + 1;
+  static constexpr int kBars = 2 * kStages + 2 + 6 + 2 * kItems + 1;
   static constexpr int OFF_MISC = OFF_BAR + kBars * 8;
-  static constexpr int kSmem = OFF_MISC + 64 + 1024;        // + alignment of the swizzled tiles
-};
-
-struct Item {
-  int q0, qn;  // the sequence's first query row and its number of query rows (tokens)
-  int k0, kn;  // first key row and number of keys
-  int tok0;    // first token of the CTA's two row tiles
-  int lo, hi;  // key tiles [lo, hi)
+  static constexpr int OFF_ITEM = OFF_MISC + 16;
+  static constexpr int kSmem = OFF_ITEM + kItems * int(sizeof(Item)) + 1024;  // + alignment of the swizzled tiles
 };
 
 // ---------------------------------------------------------------------------
-// PREFIX = false: packed prompts.  PREFIX = true: single-token rows over the pages of their group's prefix, keys split over
-// gridDim.z; shares (m, l, o) go to the workspace and are joined by the decode combine.
+// PREFIX = false: packed prompts.  PREFIX = true: single-token rows over the pages of their group's prefix, keys
+// split `splits` ways; shares (m, l, o) go to the workspace and are joined by the decode join.
+//
+// Persistent: CTA c takes the items c, 2N - 1 - c, 2N + c, ... (back and forth, so that with items in
+// descending size no CTA gets the large end of every wave).  The TMA warp finds the items and hands them
+// to the others through a small ring, so the next item's loads and first S run under this one's tail.
 // ---------------------------------------------------------------------------
 template <typename T, int D, bool PREFIX>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -137,189 +227,224 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int kvh = blockIdx.y;
   const int G = p.group, tpt = p.tpt;
 
   const uint32_t bar0 = smem_u32(smem + C::OFF_BAR);
-  const uint32_t q_full = bar0;
-  auto kv_full = [&](int s) { return bar0 + 8u * (1 + s); };
-  auto kv_empty = [&](int s) { return bar0 + 8u * (1 + C::kStages + s); };
-  auto s_full = [&](int t) { return bar0 + 8u * (1 + 2 * C::kStages + t); };
-  auto p_full = [&](int t) { return bar0 + 8u * (3 + 2 * C::kStages + t); };
-  auto o_full = [&](int t) { return bar0 + 8u * (5 + 2 * C::kStages + t); };
-  const uint32_t mma_done = bar0 + 8u * (7 + 2 * C::kStages);
+  auto kv_full = [&](int s) { return bar0 + 8u * s; };
+  auto kv_empty = [&](int s) { return bar0 + 8u * (C::kStages + s); };
+  constexpr int kB = 2 * C::kStages;
+  const uint32_t q_full = bar0 + 8u * kB, q_empty = bar0 + 8u * (kB + 1);
+  auto s_full = [&](int t) { return bar0 + 8u * (kB + 2 + t); };
+  auto p_full = [&](int t) { return bar0 + 8u * (kB + 4 + t); };
+  auto o_full = [&](int t) { return bar0 + 8u * (kB + 6 + t); };
+  auto item_full = [&](int i) { return bar0 + 8u * (kB + 8 + i); };
+  auto item_empty = [&](int i) { return bar0 + 8u * (kB + 8 + kItems + i); };
+  const uint32_t mma_done = bar0 + 8u * (kB + 8 + 2 * kItems);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
-  Item* item_s = reinterpret_cast<Item*>(smem + C::OFF_MISC + 8);
+  Item* items = reinterpret_cast<Item*>(smem + C::OFF_ITEM);
   const Ctl ctl{abort_flag, p.status};
 
-  if (PREFIX) pdl_trigger();  // the decode kernel may run beside this one
-
-  // ---- which sequence (group) and rows: warp 0 walks the sequences' numbers of row-tile pairs
-  if (warp == 0) {
-    const int n_seq = p.batch;
-    int base = 0;
-    Item it{0, 0, 0, 0, -1, 0, 0};
-    for (int s0 = 0; s0 < n_seq; s0 += 32) {
-      const int s = s0 + lane;
-      int qb = 0, qn = 0, kb = 0, kn = 0;
-      if (s < n_seq) {
-        qb = p.cu_q[s];
-        qn = p.cu_q[s + 1] - qb;
-        if (PREFIX) {
-          kn = p.prefix_lens[s];
-        } else {
-          kb = p.cu_k[s];
-          kn = p.cu_k[s + 1] - kb;
-        }
-        // offsets that do not describe rows of the tensors: report, and leave the sequence out
-        bool bad = qb < 0 || qn < 0 || int64_t(qb) + qn > p.total_q || kb < 0 || kn < 0 || int64_t(kb) + kn > p.total_k;
-        if (PREFIX) bad = bad || kn % p.page_size != 0;
-        if (bad) {
-          record_fault(p.status, KLC_ERR_DEVICE_FAULT, PREFIX ? 520 : 500, s);
-          qn = kn = 0;
-        }
-        if (PREFIX && kn == 0) qn = 0;
-      }
-      const int pairs = (qn + 2 * tpt - 1) / (2 * tpt);
-      int incl = pairs;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      const int excl = base + incl - pairs;
-      const bool mine = int(blockIdx.x) >= excl && int(blockIdx.x) < excl + pairs;
-      const unsigned hit = __ballot_sync(0xffffffffu, mine);
-      if (hit != 0) {
-        // a sequence's last rows see the most keys: its tiles run in descending order
-        if (mine) it = Item{qb, qn, kb, kn, (pairs - 1 - (int(blockIdx.x) - excl)) * 2 * tpt, 0x7fffffff, 0};
-        const int src = __ffs(hit) - 1;
-        it.q0 = __shfl_sync(0xffffffffu, it.q0, src);
-        it.qn = __shfl_sync(0xffffffffu, it.qn, src);
-        it.k0 = __shfl_sync(0xffffffffu, it.k0, src);
-        it.kn = __shfl_sync(0xffffffffu, it.kn, src);
-        it.tok0 = __shfl_sync(0xffffffffu, it.tok0, src);
-        it.lo = 0x7fffffff;
-        it.hi = 0;
-        break;
-      }
-      base += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    if (lane == 0) *item_s = it;
-  }
   if (tid == 32 * kWarpTma) {
-    mbar_init(q_full, 1);
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(kv_full(s), 1);
       mbar_init(kv_empty(s), 1);
     }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full(t), 1);
       mbar_init(p_full(t), kRows);
       mbar_init(o_full(t), 1);
     }
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(item_full(i), 1);
+      mbar_init(item_empty(i), 9);  // the MMA warp and eight softmax warps
+    }
     mbar_init(mma_done, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  __syncthreads();
-  if (item_s->tok0 < 0) return;  // past the last pair
+  if (PREFIX) pdl_trigger();  // the decode kernel may run beside this one
   if (warp == kWarpMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
                  "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-
-  // ---- each softmax thread's row: token, head, and the keys [jlo, jhi] it sees
-  const int t = warp >> 2;  // row tile of a softmax warp
-  const int r = tid & (kRows - 1);
-  const int tok_in = r / G, g = r - tok_in * G;
-  const int tok = item_s->tok0 + t * tpt + tok_in;
-  const bool row_ok = warp < 8 && r < tpt * G && tok < item_s->qn;
-  int jlo = 0x7fffffff, jhi = -1;
-  if (row_ok) {
-    const int pos = PREFIX ? p.lens[item_s->q0 + tok] - 1 : item_s->kn - item_s->qn + tok;
-    jhi = PREFIX ? min(pos, item_s->kn - 1) : pos;
-    jlo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-    if (jlo > jhi) jlo = 0x7fffffff, jhi = -1;
-  }
-  if (warp < 8) {
-    const int wlo = __reduce_min_sync(0xffffffffu, jlo), whi = __reduce_max_sync(0xffffffffu, jhi);
-    if (lane == 0) {
-      atomicMin(&item_s->lo, wlo);
-      atomicMax(&item_s->hi, whi + 1);
-    }
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  const Item it = *item_s;
-  int tile_lo = it.hi > 0 ? it.lo / kKeys : 0, tile_hi = it.hi > 0 ? (it.hi + kKeys - 1) / kKeys : 0;
-  if (PREFIX) {  // this CTA's share of the keys
-    const int n_all = tile_hi - tile_lo, z = blockIdx.z, nz = gridDim.z;
-    const int a = tile_lo + int(int64_t(n_all) * z / nz), b = tile_lo + int(int64_t(n_all) * (z + 1) / nz);
-    tile_lo = a;
-    tile_hi = b;
-  }
-  const int n = tile_hi - tile_lo;
+
+  // the next item of the ring for a consumer warp; false after the last one or on an abort
+  uint32_t item_no = 0;
+  auto next_item = [&](Item* it, int site) {
+    const int s = item_no % kItems;
+    bool ok = wait_bar(item_full(s), (item_no / kItems) & 1, ctl, site);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok) *it = items[s];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(item_empty(s));
+    ++item_no;
+    return ok && it->tok0 >= 0;
+  };
 
   if (warp == kWarpTma) {
-    // ---------------------------------------------------------------- loads
-    if (lane == 0 && n > 0) {
-      mbar_arrive_expect_tx(q_full, 2u * C::kChunks * uint32_t(tpt * G) * 128u);
-      for (int tt = 0; tt < 2; ++tt)
-        for (int c = 0; c < C::kChunks; ++c)
-          tma_load_3d(smem_u32(smem + C::OFF_Q + tt * C::kTile + c * (kRows * 128)), &map_q, c * 64, kvh * G,
-                      it.q0 + it.tok0 + tt * tpt, q_full);
-      uint32_t issued = 0;
-      bool ok = true;
-      for (int i = 0; i < n && ok; ++i) {
-        const int key = (tile_lo + i) * kKeys;
-        for (int kv = 0; kv < 2; ++kv, ++issued) {
-          const int s = issued % C::kStages;
-          if (!(ok = wait_bar(kv_empty(s), ((issued / C::kStages) & 1) ^ 1, ctl, 501))) break;
-          const uint32_t dst = smem_u32(smem + C::OFF_KV + s * C::kTile);
-          const CUtensorMap* map = kv ? &map_v : &map_k;
-          mbar_arrive_expect_tx(kv_full(s), uint32_t(C::kTile));
-          if (!PREFIX) {
-            for (int c = 0; c < C::kChunks; ++c)
-              tma_load_3d(dst + c * (kKeys * 128), map, c * 64, kvh, it.k0 + key, kv_full(s));
+    // ---------------------------------------------------------------- items and loads
+    int seq0 = 0;        // sequences before this one are done with
+    int64_t base = 0;    // row-tile pairs before sequence seq0
+    const int unit = p.kv_heads * (PREFIX ? p.splits : 1);  // items of a pair
+    uint32_t issued = 0, queries = 0;
+    bool ok = true;
+    for (uint32_t wave = 0; ok; ++wave) {
+      const int64_t idx = int64_t(wave) * gridDim.x + ((wave & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      const int64_t pair = idx / unit;
+      const int sub = int(idx - pair * unit);
+      Item it{0, 0, 0, 0, -1, 0, 0, 0, 0, 0};
+      for (; seq0 < p.batch; seq0 += 32) {
+        const int s = seq0 + lane;
+        int qb = 0, qn = 0, kb = 0, kn = 0;
+        if (s < p.batch) {
+          qb = p.cu_q[s];
+          qn = p.cu_q[s + 1] - qb;
+          if (PREFIX) {
+            kn = p.prefix_lens[s];
           } else {
-            // pages past the prefix, and ids that are no page of the pool, read as zeros (coordinate past the end)
-            for (int j = 0; j < kKeys; j += p.page_size) {
-              int page = int(p.pages);
-              if (key + j < it.kn) {
-                page = p.block_table[int64_t(it.q0) * p.table_stride + (key + j) / p.page_size];
-                if (page < 0 || page >= p.pages) {
-                  record_fault(p.status, KLC_ERR_DEVICE_FAULT, 521, page);
-                  page = int(p.pages);
-                }
-              }
+            kb = p.cu_k[s];
+            kn = p.cu_k[s + 1] - kb;
+          }
+          // offsets that do not describe rows of the tensors: report, and leave the sequence out
+          bool bad = qb < 0 || qn < 0 || int64_t(qb) + qn > p.total_q || kb < 0 || kn < 0 || int64_t(kb) + kn > p.total_k;
+          if (PREFIX) bad = bad || kn % p.page_size != 0;
+          if (bad) {
+            record_fault(p.status, KLC_ERR_DEVICE_FAULT, PREFIX ? 520 : 500, s);
+            qn = kn = 0;
+          }
+          if (PREFIX && kn == 0) qn = 0;
+        }
+        const int pairs = int((int64_t(qn) + 2 * tpt - 1) / (2 * tpt));
+        int incl = pairs;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += v;
+        }
+        const int64_t excl = base + incl - pairs;
+        const bool mine = pair >= excl && pair < excl + pairs;
+        const unsigned hit = __ballot_sync(0xffffffffu, mine);
+        if (hit != 0) {
+          const int src = __ffs(hit) - 1;
+          it.q0 = __shfl_sync(0xffffffffu, qb, src);
+          it.qn = __shfl_sync(0xffffffffu, qn, src);
+          it.k0 = __shfl_sync(0xffffffffu, kb, src);
+          it.kn = __shfl_sync(0xffffffffu, kn, src);
+          // a sequence's last rows see the most keys: its tiles run in descending order
+          it.tok0 = __shfl_sync(0xffffffffu, (pairs - 1 - int(pair - excl)) * 2 * tpt, src);
+          break;
+        }
+        base += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      if (it.tok0 >= 0) {
+        it.kvh = PREFIX ? sub / p.splits : sub;
+        it.z = PREFIX ? sub - it.kvh * p.splits : 0;
+        it.tiles = it.tok0 + tpt < it.qn ? 2 : 1;
+        int first, last;  // keys some row of the item sees
+        if (PREFIX) {
+          int lo = 0x7fffffff, hi = 0;
+          for (int i = it.tok0 + lane; i < min(it.tok0 + 2 * tpt, it.qn); i += 32) {
+            const int len = p.lens[it.q0 + i];
+            lo = min(lo, len);
+            hi = max(hi, len);
+          }
+          lo = __reduce_min_sync(0xffffffffu, lo);
+          hi = __reduce_max_sync(0xffffffffu, hi);
+          first = p.window > 0 ? max(0, lo - p.window) : 0;
+          last = min(hi, it.kn) - 1;
+        } else {
+          const int pos = it.kn - it.qn + it.tok0;
+          first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+          last = it.kn - it.qn + min(it.tok0 + 2 * tpt, it.qn) - 1;
+        }
+        int lo = 0, hi = 0;
+        if (last >= first) lo = first / kKeys, hi = last / kKeys + 1;
+        if (PREFIX) {  // this item's share of the keys
+          const int n = hi - lo;
+          hi = lo + int(int64_t(n) * (it.z + 1) / p.splits);
+          lo = lo + int(int64_t(n) * it.z / p.splits);
+        }
+        it.lo = lo;
+        it.n = hi - lo;
+      }
+      const int slot = wave % kItems;
+      ok = wait_bar(item_empty(slot), ((wave / kItems) & 1) ^ 1, ctl, 510);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      if (lane == 0) {
+        items[slot] = it;
+        mbar_arrive(item_full(slot));
+      }
+      if (it.tok0 < 0) break;
+      if (lane == 0) {
+        for (int i = 0; i < it.n && ok; ++i) {
+          const int key = (it.lo + i) * kKeys;
+          for (int kv = 0; kv < 2; ++kv, ++issued) {
+            const int s = issued % C::kStages;
+            if (!(ok = wait_bar(kv_empty(s), ((issued / C::kStages) & 1) ^ 1, ctl, 501))) break;
+            const uint32_t dst = smem_u32(smem + C::OFF_KV + s * C::kTile);
+            const CUtensorMap* map = kv ? &map_v : &map_k;
+            mbar_arrive_expect_tx(kv_full(s), uint32_t(C::kTile));
+            if (!PREFIX) {
               for (int c = 0; c < C::kChunks; ++c)
-                tma_load_4d(dst + c * (kKeys * 128) + j * 128, map, c * 64, 0, kvh, page, kv_full(s));
+                tma_load_3d(dst + c * (kKeys * 128), map, c * 64, it.kvh, it.k0 + key, kv_full(s));
+            } else {
+              // pages past the prefix, and ids that are no page of the pool, read as zeros (coordinate past the end)
+              for (int j = 0; j < kKeys; j += p.page_size) {
+                int page = int(p.pages);
+                if (key + j < it.kn) {
+                  page = p.block_table[int64_t(it.q0) * p.table_stride + (key + j) / p.page_size];
+                  if (page < 0 || page >= p.pages) {
+                    record_fault(p.status, KLC_ERR_DEVICE_FAULT, 521, page);
+                    page = int(p.pages);
+                  }
+                }
+                for (int c = 0; c < C::kChunks; ++c)
+                  tma_load_4d(dst + c * (kKeys * 128) + j * 128, map, c * 64, 0, it.kvh, page, kv_full(s));
+              }
+            }
+            if (i == 0 && kv == 0) {  // the item's queries, behind its first keys: they wait for the previous item's last S
+              if (!(ok = wait_bar(q_empty, (queries & 1) ^ 1, ctl, 511))) {
+                ++issued;
+                break;
+              }
+              mbar_arrive_expect_tx(q_full, uint32_t(it.tiles * C::kChunks * tpt * G) * 128u);
+              for (int tt = 0; tt < it.tiles; ++tt)
+                for (int c = 0; c < C::kChunks; ++c)
+                  tma_load_3d(smem_u32(smem + C::OFF_Q + tt * C::kTile + c * (kRows * 128)), &map_q, c * 64, it.kvh * G,
+                              it.q0 + it.tok0 + tt * tpt, q_full);
+              ++queries;
             }
           }
         }
       }
-      if (!ok) {
-        drain_wait(q_full, 0);
-        drain_ring(kv_full(0), C::kStages, issued);
-      }
+      ok = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
     }
+    if (!ok && lane == 0) {
+      if (queries > 0) drain_wait(q_full, (queries - 1) & 1);
+      drain_ring(kv_full(0), C::kStages, issued);
+    }
+    __syncwarp();
   } else if (warp == kWarpMma) {
     // ---------------------------------------------------------------- MMA
     constexpr uint32_t idesc_qk = f16_idesc<T>(kRows, kKeys, false);
     constexpr uint32_t idesc_pv = f16_idesc<T>(kRows, D, true);
     bool ok = true;
-    auto stage_ptr = [&](int s) { return smem + C::OFF_KV + s * C::kTile; };
+    auto stage_ptr = [&](uint32_t i) { return smem + C::OFF_KV + (i % C::kStages) * C::kTile; };
     auto wait_all = [&](uint32_t bar, uint32_t parity, int site) {
       const bool w = wait_bar(bar, parity, ctl, site);
       return __all_sync(0xffffffffu, w) != 0;
     };
-    auto qk = [&](int tt, int s) {  // S_tt = Q_tt K^T
-      const uint64_t a = sw128_desc(smem_u32(smem + C::OFF_Q + tt * C::kTile)), b = sw128_desc(smem_u32(stage_ptr(s)));
+    auto wait_kv = [&](uint32_t i, int site) { return wait_all(kv_full(i % C::kStages), (i / C::kStages) & 1, site); };
+    auto qk = [&](int tt, uint32_t i) {  // S_tt = Q_tt K^T
+      const uint64_t a = sw128_desc(smem_u32(smem + C::OFF_Q + tt * C::kTile)), b = sw128_desc(smem_u32(stage_ptr(i)));
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const uint64_t off = uint64_t((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4;
@@ -327,149 +452,207 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       }
       tc_commit(s_full(tt));
     };
-    auto pv = [&](int tt, int s, bool first) {  // O_tt += P_tt V
-      const uint64_t b = sw128_mn_desc(smem_u32(stage_ptr(s)), kKeys * 128);
+    auto pv = [&](int tt, uint32_t i, bool first) {  // O_tt += P_tt V
+      const uint64_t b = sw128_mn_desc(smem_u32(stage_ptr(i)), kKeys * 128);
 #pragma unroll
       for (int kk = 0; kk < kKeys / 16; ++kk)
         mma_ts(tmem + uint32_t(2 * kKeys + tt * D), tmem + uint32_t(tt * kKeys + kk * 8), b + (uint64_t(kk * 16 * 128) >> 4),
                idesc_pv, !(first && kk == 0));
     };
-    if (n > 0) {
-      ok = wait_all(q_full, 0, 502) && wait_all(kv_full(0), 0, 503);
+    uint32_t used = 0, queries = 0, steps[2] = {0, 0};  // ring stages, items with keys, key tiles per row tile
+    Item it;
+    while (ok && next_item(&it, 512)) {
+      const int n = it.n, last_tt = it.tiles - 1;
+      if (n == 0) continue;
+      if (!(ok = wait_kv(used, 503) && wait_all(q_full, queries & 1, 502))) break;
+      ++queries;
       tc_fence_after();
-      if (ok && lane == 0) {
-        qk(0, 0);
-        qk(1, 0);
-        tc_commit(kv_empty(0));
+      if (lane == 0) {
+        for (int tt = 0; tt < it.tiles; ++tt) qk(tt, used);
+        tc_commit(kv_empty(used % C::kStages));
+        if (n == 1) tc_commit(q_empty);
       }
+      __syncwarp();
       for (int i = 0; i < n && ok; ++i) {
-        const int iv = 2 * i + 1, sv = iv % C::kStages, ik = 2 * i + 2, sk = ik % C::kStages;
+        const uint32_t iv = used + 2 * i + 1, ik = iv + 1;
         const bool more = i + 1 < n;
-        if (!(ok = wait_all(kv_full(sv), (iv / C::kStages) & 1, 504))) break;
+        if (!(ok = wait_kv(iv, 504))) break;
         if (!PREFIX) {
           // value rows past the sequence's last key belong to someone else: 0 * anything finite or not must be 0
-          const int valid = it.kn - (tile_lo + i) * kKeys;
+          const int valid = it.kn - (it.lo + i) * kKeys;
           if (valid < kKeys) {
             for (int j = valid * 8 + lane; j < kKeys * 8; j += 32)
 #pragma unroll
               for (int c = 0; c < C::kChunks; ++c)
-                *reinterpret_cast<uint4*>(stage_ptr(sv) + c * (kKeys * 128) + j * 16) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(stage_ptr(iv) + c * (kKeys * 128) + j * 16) = make_uint4(0, 0, 0, 0);
             fence_proxy_async();
             __syncwarp();
           }
         }
-        for (int tt = 0; tt < 2 && ok; ++tt) {
-          if (!(ok = wait_all(p_full(tt), i & 1, 505 + tt))) break;
+        for (int tt = 0; tt < it.tiles; ++tt) {
+          if (!(ok = wait_all(p_full(tt), steps[tt] & 1, 505 + tt))) break;
+          ++steps[tt];
           tc_fence_after();
           if (lane == 0) {
-            pv(tt, sv, i == 0);
-            if (tt == 1) tc_commit(kv_empty(sv));
+            pv(tt, iv, i == 0);
+            if (tt == last_tt) tc_commit(kv_empty(iv % C::kStages));
             if (!more) tc_commit(o_full(tt));
           }
           if (more) {
-            if (tt == 0 && !(ok = wait_all(kv_full(sk), (ik / C::kStages) & 1, 507))) break;
+            if (tt == 0 && !(ok = wait_kv(ik, 507))) break;
             tc_fence_after();
             if (lane == 0) {
-              qk(tt, sk);
-              if (tt == 1) tc_commit(kv_empty(sk));
+              qk(tt, ik);
+              if (tt == last_tt) {
+                tc_commit(kv_empty(ik % C::kStages));
+                if (i + 2 == n) tc_commit(q_empty);
+              }
             }
           }
           __syncwarp();
         }
       }
-      if (!ok && lane == 0) {  // aborting: no MMA may still be in flight when TMEM is freed
-        tc_commit(mma_done);
-        drain_wait(mma_done, 0);
-      }
-      __syncwarp();
+      used += 2 * uint32_t(n);
     }
+    if (*abort_flag && lane == 0) {  // no MMA may still be in flight when TMEM is freed
+      tc_commit(mma_done);
+      drain_wait(mma_done, 0);
+    }
+    __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax
+    const int t = warp >> 2;  // row tile
+    const int r = tid & (kRows - 1);
+    const int tok_in = r / G, g = r - tok_in * G;
     const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + lane_base + uint32_t(t * kKeys);
     const uint32_t o_col = tmem + lane_base + uint32_t(2 * kKeys + t * D);
-    float m = -INFINITY, l = 0.f;  // m: reference maximum (log2 units) of the stored P and O
-    bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      ok = wait_bar(s_full(t), i & 1, ctl, 508);
-      if (!(ok = __all_sync(0xffffffffu, ok))) break;
-      tc_fence_after();
-      // The row is read twice, 32 columns at a time: for its maximum, then for the exponentials
-      // (TMEM reads are cheap next to keeping 128 scores in registers).
-      const int kb = (tile_lo + i) * kKeys;
-      const bool masked = __any_sync(0xffffffffu, kb < jlo || kb + kKeys - 1 > jhi);
-      const int ja = jlo - kb, jb = jhi - kb;
-      auto load_scores = [&](int c, float* s) {
-        tmem_ld32(s_col + uint32_t(32 * c), s);
-        tmem_wait_ld32(s);
+    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+    uint32_t steps = 0, ends = 0;
+    Item it;
+    while (next_item(&it, 513)) {
+      if (t >= it.tiles) continue;  // no row in this tile
+      // the row and the keys [jlo, jhi] it sees
+      const int tok = it.tok0 + t * tpt + tok_in;
+      const bool row_ok = r < tpt * G && tok < it.qn;
+      int jlo = 0x7fffffff, jhi = -1;
+      if (row_ok) {
+        const int pos = PREFIX ? p.lens[it.q0 + tok] - 1 : it.kn - it.qn + tok;
+        jhi = PREFIX ? min(pos, it.kn - 1) : pos;
+        jlo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+        if (jlo > jhi) jlo = 0x7fffffff, jhi = -1;
+      }
+      // the row reaches these tiles whole: rows that are not there do not make a tile a boundary one
+      const int wlo = __reduce_max_sync(0xffffffffu, row_ok ? jlo : 0), whi = __reduce_min_sync(0xffffffffu, row_ok ? jhi : 0x7fffffff);
+      float m = -INFINITY, l = 0.f;  // m: reference maximum (log2 units) of the stored P and O
+      bool ok = true;
+      for (int i = 0; i < it.n; ++i, ++steps) {
+        ok = wait_bar(s_full(t), steps & 1, ctl, 508);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        tc_fence_after();
+        const int kb = (it.lo + i) * kKeys;
+        const bool masked = kb < wlo || kb + kKeys - 1 > whi;
+        const int ja = jlo - kb, jb = jhi - kb;
+        // Columns 0-63 are read twice and 64-127 kept (all 128 would not fit the registers).
+        float sa[64], sb[64];
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tmem_ld64(s_col, sa);
+        tmem_wait_ld64(sa);
+        tmem_ld64(s_col + 64, sb);
         if (masked) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) s[j] = (32 * c + j >= ja && 32 * c + j <= jb) ? s[j] : -INFINITY;
+          for (int j = 0; j < 64; ++j) sa[j] = (j >= ja && j <= jb) ? sa[j] : -INFINITY;
         }
-      };
-      float mx = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float s[32];
-        load_scores(c, s);
+        for (int j = 0; j < 64; j += 2) mx[(j >> 1) & 3] = max3_nan(mx[(j >> 1) & 3], sa[j], sa[j + 1]);
+        tmem_wait_ld64(sb);
+        if (masked) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) mx = fmaxf(mx, s[j]);
-      }
-      const float m_new = fmaxf(m, mx * p.scale_log2);
-      const bool grow = m_new > m + kRescaleLog2 || (m == -INFINITY && m_new > m);
-      if (__any_sync(0xffffffffu, grow)) {
-        const float f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - m_new)) : 1.f;
-        if (grow) {
-          m = m_new;
-          l *= f;
+          for (int j = 0; j < 64; ++j) sb[j] = (64 + j >= ja && 64 + j <= jb) ? sb[j] : -INFINITY;
         }
-        if (i > 0) {  // S of this tile is issued behind the previous P V: O is complete
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            float o[32];
-            tmem_ld32(o_col + uint32_t(32 * c), o);
-            tmem_wait_ld32(o);
+        for (int j = 0; j < 64; j += 2) mx[(j >> 1) & 3] = max3_nan(mx[(j >> 1) & 3], sb[j], sb[j + 1]);
+        const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;
+        // the reference moves when the maximum has grown by more than 2^8 (or to a NaN)
+        const bool grow = row_ok && (m == -INFINITY ? top != -INFINITY : !(top <= m + kRescaleLog2));
+        if (__any_sync(0xffffffffu, grow)) {
+          const float f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
+          if (grow) {
+            m = top;
+            l *= f;
+          }
+          if (i > 0) {  // S of this tile is issued behind the previous P V: O is complete
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] *= f;
-            tmem_st32(o_col + uint32_t(32 * c), reinterpret_cast<const uint32_t*>(o));
+            for (int c = 0; c < D / 16; ++c) {
+              float o[16];
+              tmem_ld16f(o_col + uint32_t(16 * c), o);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] *= f;
+              tmem_st16(o_col + uint32_t(16 * c), reinterpret_cast<const uint32_t*>(o));
+            }
           }
         }
-      }
-      const float mref = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        float s0[32];
+        tmem_ld32(s_col, s0);
+        const float mref = m == -INFINITY ? 0.f : m;
+        const float2 off2 = make_float2(-mref, -mref);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // numerators of 32 scores, packed; boundary tiles use the special-function unit alone (it gives an exact 0)
+        auto numerators = [&](const float* s, uint32_t* pk, auto whole) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float s[32];
-        uint32_t pk[16];
-        load_scores(c, s);
+          for (int j = 0; j < 32; j += 2) {
+            const float2 x = fma2(make_float2(s[j], s[j + 1]), scale2, off2);
+            float2 e;
+            if (decltype(whole)::value && (j >> 1) % 8 < C::kFmaPairs) e = exp2_fma<T>(x);
+            else e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+            sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], e);
+            pk[j >> 1] = Elem<T>::pack(e.x, e.y);
+          }
+        };
+        auto write_p = [&](auto whole) {
+          auto hide = [&](float* s, int c) {
+            if (!decltype(whole)::value) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const float e0 = exp2_approx(fmaf(s[j], p.scale_log2, -mref));
-          const float e1 = exp2_approx(fmaf(s[j + 1], p.scale_log2, -mref));
-          sum[j & 2] += e0;
-          sum[(j & 2) + 1] += e1;
-          pk[j / 2] = Elem<T>::pack(e0, e1);
-        }
-        tmem_st16(s_col + uint32_t(16 * c), pk);  // over columns whose scores have been read
+              for (int j = 0; j < 32; ++j) s[j] = (c + j >= ja && c + j <= jb) ? s[j] : -INFINITY;
+            }
+          };
+          uint32_t pb[32], pa[16];
+          numerators(sb, pb, whole);
+          numerators(sb + 32, pb + 16, whole);
+          tmem_wait_ld32(s0);
+          float s1[32];
+          tmem_ld32(s_col + 32, s1);
+          hide(s0, 0);
+          numerators(s0, pa, whole);
+          tmem_wait_ld32(s1);
+          tmem_st16(s_col, pa);  // P over columns whose scores have been read
+          hide(s1, 32);
+          numerators(s1, pa, whole);
+          tmem_st16(s_col + 16, pa);
+          tmem_st32(s_col + 32, pb);
+        };
+        if (masked) write_p(std::false_type{});
+        else write_p(std::true_type{});
+        const float2 both = add2(sum[0], sum[1]);
+        l += both.x + both.y;
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(p_full(t));
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(p_full(t));
-    }
-    // ---- epilogue: the row's output
-    if (ok && n > 0) {
-      ok = wait_bar(o_full(t), 0, ctl, 509);
-      ok = __all_sync(0xffffffffu, ok);
-      tc_fence_after();
-    }
-    if (ok) {
+      // ---- epilogue: the row's output
+      if (ok && it.n > 0) {
+        ok = wait_bar(o_full(t), ends & 1, ctl, 509);
+        ok = __all_sync(0xffffffffu, ok);
+        ++ends;
+        tc_fence_after();
+      }
+      if (!ok) break;
       const int64_t row = int64_t(it.q0) + tok;
-      const int head = kvh * G + g;
+      const int head = it.kvh * G + g;
       if (PREFIX) {
-        const int64_t slot = (int64_t(blockIdx.z) * p.total_q + row) * p.heads + head;
+        const int64_t slot = (int64_t(it.z) * p.total_q + row) * p.heads + head;
         if (row_ok) p.part_ml[slot] = make_float2(m, l);
-        if (n > 0) {
+        if (it.n > 0) {
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             float o[32];
@@ -493,7 +676,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
-          if (n > 0) {
+          if (it.n > 0) {
             tmem_ld32(o_col + uint32_t(32 * c), o);
             tmem_wait_ld32(o);
           } else {
@@ -524,21 +707,21 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 }
 
 template <typename T, int D, bool PREFIX>
-int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& p, dim3 grid, cudaStream_t s) {
+int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& p, int64_t items, cudaStream_t s) {
   auto kernel = attn_tc_kernel<T, D, PREFIX>;
   KLC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
-  kernel<<<grid, kThreads, Cfg<D>::kSmem, s>>>(mq, mk, mv, p);
+  kernel<<<unsigned(std::min<int64_t>(items, sm_count())), kThreads, Cfg<D>::kSmem, s>>>(mq, mk, mv, p);
   KLC_LAUNCH_CHECK(PREFIX ? "attn_prefix" : "attn_prompt");
   return KLC_OK;
 }
 
 template <bool PREFIX>
 int launch_typed(int dtype, int head_dim, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                 const TcParams& p, dim3 grid, cudaStream_t s) {
+                 const TcParams& p, int64_t items, cudaStream_t s) {
   if (dtype == KLC_BF16)
-    return head_dim == 64 ? launch<__nv_bfloat16, 64, PREFIX>(mq, mk, mv, p, grid, s)
-                          : launch<__nv_bfloat16, 128, PREFIX>(mq, mk, mv, p, grid, s);
-  return head_dim == 64 ? launch<__half, 64, PREFIX>(mq, mk, mv, p, grid, s) : launch<__half, 128, PREFIX>(mq, mk, mv, p, grid, s);
+    return head_dim == 64 ? launch<__nv_bfloat16, 64, PREFIX>(mq, mk, mv, p, items, s)
+                          : launch<__nv_bfloat16, 128, PREFIX>(mq, mk, mv, p, items, s);
+  return head_dim == 64 ? launch<__half, 64, PREFIX>(mq, mk, mv, p, items, s) : launch<__half, 128, PREFIX>(mq, mk, mv, p, items, s);
 }
 
 CUtensorMapDataType map_type(int dtype) {
@@ -582,6 +765,8 @@ int launch_prefix(const klc_attn_dims& dims, const DecodeParams& d, const void* 
   p.total_q = d.batch;
   p.total_k = int64_t(d.table_width) * d.page_size;
   p.heads = d.heads;
+  p.kv_heads = d.kv_heads;
+  p.splits = d.splits;
   p.group = d.group;
   p.tpt = kRows / d.group;
   p.scale_log2 = d.scale_log2;
@@ -602,8 +787,7 @@ int launch_prefix(const klc_attn_dims& dims, const DecodeParams& d, const void* 
   if (st != KLC_OK) return st;
   const int tok = 2 * p.tpt;
   const int pairs = d.groups == 1 ? (d.batch + tok - 1) / tok : std::min(d.batch, d.batch / tok + d.groups);
-  return launch_typed<true>(dims.dtype, dims.head_dim, mq, mk, mv, p,
-                            dim3(unsigned(pairs), unsigned(d.kv_heads), unsigned(d.splits)), stream);
+  return launch_typed<true>(dims.dtype, dims.head_dim, mq, mk, mv, p, int64_t(pairs) * d.kv_heads * d.splits, stream);
 }
 
 }  // namespace attn
@@ -645,6 +829,7 @@ extern "C" int klc_attn_prompt(const klc_attn_dims* dims, const void* q, int64_t
   p.total_q = q_tokens;
   p.total_k = k_tokens;
   p.heads = dims->heads;
+  p.kv_heads = dims->kv_heads;
   p.group = G;
   p.tpt = kRows / G;
   p.scale_log2 = dims->scale * kLog2e;
@@ -662,5 +847,5 @@ extern "C" int klc_attn_prompt(const klc_attn_dims* dims, const void* q, int64_t
   if ((st = rows_map(&mv, dims->dtype, d, v, kt, dims->kv_heads, v_token_stride, v_head_stride, 1, kKeys)) != KLC_OK) return st;
   // pairs of row tiles: sum over sequences of ceil(len / (2 tpt)), at most this
   const int64_t gx = q_tokens / (2 * p.tpt) + std::min<int64_t>(batch, q_tokens);
-  return launch_typed<false>(dims->dtype, d, mq, mk, mv, p, dim3(unsigned(gx), unsigned(dims->kv_heads)), as_stream(stream));
+  return launch_typed<false>(dims->dtype, d, mq, mk, mv, p, gx * dims->kv_heads, as_stream(stream));
 }
