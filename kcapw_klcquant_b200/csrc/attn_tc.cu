@@ -157,19 +157,30 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
-// D[tmem] (+)= A[tmem or smem] * B[smem]
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// D[tmem] (+)= A[tmem or smem] * B[smem].  The whole warp runs these with the same operands and one elected lane
+// (always the same) issues: operands stay in uniform registers.  Behind a per-lane branch each instruction took
+// about 130 cycles to issue, three times what an M = 128, N = 64 product takes to run.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                       uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %6, 0;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 b;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void commit_elected(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
       : "memory");
 }
 
@@ -180,11 +191,12 @@ __device__ __forceinline__ constexpr uint32_t f16_idesc(int m, int n, bool b_mn_
          (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
 
-// MN-major operand, 128-byte swizzle: rows of 64 contiguous MN elements, one row per K; eight-row
-// groups 1024 bytes apart along K (SBO), the next 64 MN elements `mn_stride` bytes on (LBO).
-__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t mn_stride) {
-  return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(mn_stride >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
-         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+// Shared-memory descriptors with 128-byte swizzle and eight-row groups 1024 bytes apart, as two words; the low word is
+// the address and a stride, and only it changes from step to step.  K-major: rows of 64 K elements.  MN-major: rows of
+// 64 MN elements, one row per K, the next 64 MN elements `mn_stride` bytes on.
+constexpr uint32_t kDescHi = uint32_t(1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t mn_stride) {
+  return ((saddr & 0x3FFFFu) >> 4) | ((mn_stride == 0 ? 1u : mn_stride >> 4) << 16);
 }
 
 struct Item {
@@ -226,7 +238,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   using C = Cfg<D>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int G = p.group, tpt = p.tpt;
 
   const uint32_t bar0 = smem_u32(smem + C::OFF_BAR);
@@ -274,7 +286,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_holder;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_holder, 0);
 
   // the next item of the ring for a consumer warp; false after the last one or on an abort
   uint32_t item_no = 0;
@@ -443,20 +455,22 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       return __all_sync(0xffffffffu, w) != 0;
     };
     auto wait_kv = [&](uint32_t i, int site) { return wait_all(kv_full(i % C::kStages), (i / C::kStages) & 1, site); };
+    const uint32_t q_lo = desc_lo(smem_u32(smem + C::OFF_Q), 0), k_lo = desc_lo(smem_u32(smem + C::OFF_KV), 0);
+    const uint32_t v_lo = desc_lo(smem_u32(smem + C::OFF_KV), kKeys * 128);
     auto qk = [&](int tt, uint32_t i) {  // S_tt = Q_tt K^T
-      const uint64_t a = sw128_desc(smem_u32(smem + C::OFF_Q + tt * C::kTile)), b = sw128_desc(smem_u32(stage_ptr(i)));
+      const uint32_t a = q_lo + uint32_t(tt * (C::kTile >> 4)), b = k_lo + (i % C::kStages) * (C::kTile >> 4);
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        const uint64_t off = uint64_t((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4;
-        mma_ss(tmem + uint32_t(tt * kKeys), a + off, b + off, idesc_qk, kk > 0);
+        const uint32_t off = uint32_t((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4;
+        mma_ss(tmem + uint32_t(tt * kKeys), a + off, kDescHi, b + off, kDescHi, idesc_qk, kk > 0);
       }
-      tc_commit(s_full(tt));
+      commit_elected(s_full(tt));
     };
     auto pv = [&](int tt, uint32_t i, bool first) {  // O_tt += P_tt V
-      const uint64_t b = sw128_mn_desc(smem_u32(stage_ptr(i)), kKeys * 128);
+      const uint32_t b = v_lo + (i % C::kStages) * (C::kTile >> 4);
 #pragma unroll
       for (int kk = 0; kk < kKeys / 16; ++kk)
-        mma_ts(tmem + uint32_t(2 * kKeys + tt * D), tmem + uint32_t(tt * kKeys + kk * 8), b + (uint64_t(kk * 16 * 128) >> 4),
+        mma_ts(tmem + uint32_t(2 * kKeys + tt * D), tmem + uint32_t(tt * kKeys + kk * 8), b + (uint32_t(kk * 16 * 128) >> 4), kDescHi,
                idesc_pv, !(first && kk == 0));
     };
     uint32_t used = 0, queries = 0, steps[2] = {0, 0};  // ring stages, items with keys, key tiles per row tile
@@ -467,12 +481,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       if (!(ok = wait_kv(used, 503) && wait_all(q_full, queries & 1, 502))) break;
       ++queries;
       tc_fence_after();
-      if (lane == 0) {
-        for (int tt = 0; tt < it.tiles; ++tt) qk(tt, used);
-        tc_commit(kv_empty(used % C::kStages));
-        if (n == 1) tc_commit(q_empty);
-      }
-      __syncwarp();
+      for (int tt = 0; tt < it.tiles; ++tt) qk(tt, used);
+      commit_elected(kv_empty(used % C::kStages));
+      if (n == 1) commit_elected(q_empty);
       for (int i = 0; i < n && ok; ++i) {
         const uint32_t iv = used + 2 * i + 1, ik = iv + 1;
         const bool more = i + 1 < n;
@@ -489,36 +500,34 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             __syncwarp();
           }
         }
-        for (int tt = 0; tt < it.tiles; ++tt) {
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+          if (tt > last_tt) break;
           if (!(ok = wait_all(p_full(tt), steps[tt] & 1, 505 + tt))) break;
           ++steps[tt];
           tc_fence_after();
-          if (lane == 0) {
-            pv(tt, iv, i == 0);
-            if (tt == last_tt) tc_commit(kv_empty(iv % C::kStages));
-            if (!more) tc_commit(o_full(tt));
-          }
+          pv(tt, iv, i == 0);
+          if (tt == last_tt) commit_elected(kv_empty(iv % C::kStages));
+          if (!more) commit_elected(o_full(tt));
           if (more) {
             if (tt == 0 && !(ok = wait_kv(ik, 507))) break;
             tc_fence_after();
-            if (lane == 0) {
-              qk(tt, ik);
-              if (tt == last_tt) {
-                tc_commit(kv_empty(ik % C::kStages));
-                if (i + 2 == n) tc_commit(q_empty);
-              }
+            qk(tt, ik);
+            if (tt == last_tt) {
+              commit_elected(kv_empty(ik % C::kStages));
+              if (i + 2 == n) commit_elected(q_empty);
             }
           }
-          __syncwarp();
         }
       }
       used += 2 * uint32_t(n);
     }
-    if (*abort_flag && lane == 0) {  // no MMA may still be in flight when TMEM is freed
-      tc_commit(mma_done);
-      drain_wait(mma_done, 0);
-    }
     __syncwarp();
+    if (__any_sync(0xffffffffu, *abort_flag != 0)) {  // no MMA may still be in flight when TMEM is freed
+      commit_elected(mma_done);
+      if (lane == 0) drain_wait(mma_done, 0);
+      __syncwarp();
+    }
   } else {
     // ---------------------------------------------------------------- softmax
     const int t = warp >> 2;  // row tile
