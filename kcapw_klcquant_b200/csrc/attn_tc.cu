@@ -11,8 +11,8 @@
 // sequences fill tiles that 128 tokens of one head would not.  Keys come in
 // tiles of 128.  Warps:
 //   0-3, 4-7  softmax of row tile 0 / 1, one row per thread (TMEM lane = row)
-//   8         MMA issuer (one thread); zeroes value rows past the keys' end
-//   9         TMA producer (queries once, then a ring of key and value tiles)
+//   8, 10     MMA issuer of row tile 0 / 1 (one thread); zeroes value rows past the keys' end
+//   9         finds the items; TMA producer (queries, then a ring of key and value tiles)
 // Per key tile and row tile: S = Q K^T into TMEM (128 fp32 columns), the
 // softmax thread reads its row, writes P as 16-bit pairs over S, and O += P V
 // reads P from TMEM.  The tensor pipe works on one row tile while the other is
@@ -34,10 +34,16 @@ using namespace tc;
 
 namespace {
 
+// wait_bar with everything but the first try out of line (the waits are many, and code size costs here)
+__device__ __noinline__ bool wait_bar_long(uint32_t bar, uint32_t parity, const Ctl& c, int site) { return wait_bar(bar, parity, c, site); }
+__device__ __forceinline__ bool wait_bar_short(uint32_t bar, uint32_t parity, const Ctl& c, int site) {
+  return mbar_try_wait(bar, parity) || wait_bar_long(bar, parity, c, site);
+}
+
 constexpr int kRows = 128;     // rows of a row tile (TMEM lanes)
 constexpr int kKeys = 128;     // keys of a key tile
-constexpr int kThreads = 320;  // 8 softmax warps, MMA warp, TMA warp
-constexpr int kWarpMma = 8, kWarpTma = 9;
+constexpr int kThreads = 352;  // 8 softmax warps, an MMA warp for each row tile, TMA warp
+constexpr int kWarpMma0 = 8, kWarpTma = 9, kWarpMma1 = 10;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;
 constexpr int kItems = 2;      // ring of items between the TMA warp and the others
@@ -157,30 +163,31 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
-// D[tmem] (+)= A[tmem or smem] * B[smem].  The whole warp runs these with the same operands and one elected lane
-// (always the same) issues: operands stay in uniform registers.  Behind a per-lane branch each instruction took
-// about 130 cycles to issue, three times what an M = 128, N = 64 product takes to run.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+// D[tmem] (+)= A[tmem or smem] * B[smem].  The whole warp runs these with the same operands and one lane (`lead`)
+// issues: operands stay in uniform registers.  Behind a per-lane branch each instruction took
+// about 130 cycles to issue, four times what an M = 128, N = 64 product takes to run.
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
                                        uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %6, 0;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
+      "setp.ne.u32 e, %6, 0;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc), "r"(lead)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p, e;\n\t.reg .b64 b;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "setp.ne.u32 e, %6, 0;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
+      "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc), "r"(lead)
       : "memory");
 }
-__device__ __forceinline__ void commit_elected(uint32_t bar) {
+__device__ __forceinline__ void commit_lead(uint32_t lead, uint32_t bar) {
   asm volatile(
-      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+      "{\n\t.reg .pred e;\n\tsetp.ne.u32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(lead)
       : "memory");
 }
 
@@ -212,12 +219,17 @@ template <int D>
 struct Cfg {
   static constexpr int kChunks = D / 64;                    // 128-byte columns of a head's row
   static constexpr int kTile = kKeys * D * 2;               // bytes of a query, key or value tile
-  static constexpr int kStages = D == 64 ? 10 : 5;          // ring of key and value tiles: 160 KB
+  static constexpr int kStages = D == 64 ? 5 : 2;           // ring of key and value tiles: 160 / 128 KB
   static constexpr int kFmaPairs = D == 64 ? 3 : 2;         // of 8 pairs of exponentials, on the FMA pipe
+  // TMEM columns: S 0-255, O behind it.  D = 64 leaves room for P, so the next S can be made while this one's
+  // exponentials are; with D = 128 P lies over the upper half of S, which is in registers by then.
+  static constexpr bool kOwnP = D == 64;
+  static constexpr int kColO = 2 * kKeys;
+  static constexpr int kColP = kOwnP ? kColO + 2 * D : kKeys / 2, kStepP = kOwnP ? kKeys / 2 : kKeys;
   static constexpr int OFF_Q = 0;                           // two row tiles
   static constexpr int OFF_KV = 2 * kTile;
-  static constexpr int OFF_BAR = OFF_KV + kStages * kTile;
-  static constexpr int kBars = 2 * kStages + 2 + 6 + 2 * kItems + 1;
+  static constexpr int OFF_BAR = OFF_KV + kStages * 2 * kTile;
+  static constexpr int kBars = 2 * kStages + 2 + 8 + 2 * kItems + 1;
   static constexpr int OFF_MISC = OFF_BAR + kBars * 8;
   static constexpr int OFF_ITEM = OFF_MISC + 16;
   static constexpr int kSmem = OFF_ITEM + kItems * int(sizeof(Item)) + 1024;  // + alignment of the swizzled tiles
@@ -249,9 +261,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   auto s_full = [&](int t) { return bar0 + 8u * (kB + 2 + t); };
   auto p_full = [&](int t) { return bar0 + 8u * (kB + 4 + t); };
   auto o_full = [&](int t) { return bar0 + 8u * (kB + 6 + t); };
-  auto item_full = [&](int i) { return bar0 + 8u * (kB + 8 + i); };
-  auto item_empty = [&](int i) { return bar0 + 8u * (kB + 8 + kItems + i); };
-  const uint32_t mma_done = bar0 + 8u * (kB + 8 + 2 * kItems);
+  auto s_free = [&](int t) { return bar0 + 8u * (kB + 8 + t); };
+  auto item_full = [&](int i) { return bar0 + 8u * (kB + 10 + i); };
+  auto item_empty = [&](int i) { return bar0 + 8u * (kB + 10 + kItems + i); };
+  const uint32_t mma_done = bar0 + 8u * (kB + 10 + 2 * kItems);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
   Item* items = reinterpret_cast<Item*>(smem + C::OFF_ITEM);
@@ -260,25 +273,26 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   if (tid == 32 * kWarpTma) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(kv_full(s), 1);
-      mbar_init(kv_empty(s), 1);
+      mbar_init(kv_empty(s), 2);  // both MMA warps
     }
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 2);
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full(t), 1);
       mbar_init(p_full(t), kRows);
+      mbar_init(s_free(t), kRows);
       mbar_init(o_full(t), 1);
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(item_full(i), 1);
-      mbar_init(item_empty(i), 9);  // the MMA warp and eight softmax warps
+      mbar_init(item_empty(i), 10);  // the MMA and the softmax warps
     }
-    mbar_init(mma_done, 1);
+    mbar_init(mma_done, 2);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (PREFIX) pdl_trigger();  // the decode kernel may run beside this one
-  if (warp == kWarpMma) {
+  if (warp == kWarpMma0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
                  "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -292,7 +306,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   uint32_t item_no = 0;
   auto next_item = [&](Item* it, int site) {
     const int s = item_no % kItems;
-    bool ok = wait_bar(item_full(s), (item_no / kItems) & 1, ctl, site);
+    bool ok = wait_bar_short(item_full(s), (item_no / kItems) & 1, ctl, site);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) *it = items[s];
     __syncwarp();
@@ -388,7 +402,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         it.n = hi - lo;
       }
       const int slot = wave % kItems;
-      ok = wait_bar(item_empty(slot), ((wave / kItems) & 1) ^ 1, ctl, 510);
+      ok = wait_bar_short(item_empty(slot), ((wave / kItems) & 1) ^ 1, ctl, 510);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       if (lane == 0) {
         items[slot] = it;
@@ -396,14 +410,13 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       }
       if (it.tok0 < 0) break;
       if (lane == 0) {
-        for (int i = 0; i < it.n && ok; ++i) {
-          const int key = (it.lo + i) * kKeys;
-          for (int kv = 0; kv < 2; ++kv, ++issued) {
-            const int s = issued % C::kStages;
-            if (!(ok = wait_bar(kv_empty(s), ((issued / C::kStages) & 1) ^ 1, ctl, 501))) break;
-            const uint32_t dst = smem_u32(smem + C::OFF_KV + s * C::kTile);
+        for (int i = 0; i < it.n; ++i, ++issued) {
+          const int key = (it.lo + i) * kKeys, s = issued % C::kStages;
+          if (!(ok = wait_bar_short(kv_empty(s), ((issued / C::kStages) & 1) ^ 1, ctl, 501))) break;
+          mbar_arrive_expect_tx(kv_full(s), 2u * uint32_t(C::kTile));
+          for (int kv = 0; kv < 2; ++kv) {
+            const uint32_t dst = smem_u32(smem + C::OFF_KV + (2 * s + kv) * C::kTile);
             const CUtensorMap* map = kv ? &map_v : &map_k;
-            mbar_arrive_expect_tx(kv_full(s), uint32_t(C::kTile));
             if (!PREFIX) {
               for (int c = 0; c < C::kChunks; ++c)
                 tma_load_3d(dst + c * (kKeys * 128), map, c * 64, it.kvh, it.k0 + key, kv_full(s));
@@ -422,18 +435,18 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                   tma_load_4d(dst + c * (kKeys * 128) + j * 128, map, c * 64, 0, it.kvh, page, kv_full(s));
               }
             }
-            if (i == 0 && kv == 0) {  // the item's queries, behind its first keys: they wait for the previous item's last S
-              if (!(ok = wait_bar(q_empty, (queries & 1) ^ 1, ctl, 511))) {
-                ++issued;
-                break;
-              }
-              mbar_arrive_expect_tx(q_full, uint32_t(it.tiles * C::kChunks * tpt * G) * 128u);
-              for (int tt = 0; tt < it.tiles; ++tt)
-                for (int c = 0; c < C::kChunks; ++c)
-                  tma_load_3d(smem_u32(smem + C::OFF_Q + tt * C::kTile + c * (kRows * 128)), &map_q, c * 64, it.kvh * G,
-                              it.q0 + it.tok0 + tt * tpt, q_full);
-              ++queries;
+          }
+          if (i == 0) {  // the item's queries, behind its first keys: they wait for the previous item's last S
+            if (!(ok = wait_bar_short(q_empty, (queries & 1) ^ 1, ctl, 511))) {
+              ++issued;
+              break;
             }
+            mbar_arrive_expect_tx(q_full, uint32_t(it.tiles * C::kChunks * tpt * G) * 128u);
+            for (int tt = 0; tt < it.tiles; ++tt)
+              for (int c = 0; c < C::kChunks; ++c)
+                tma_load_3d(smem_u32(smem + C::OFF_Q + tt * C::kTile + c * (kRows * 128)), &map_q, c * 64, it.kvh * G,
+                            it.q0 + it.tok0 + tt * tpt, q_full);
+            ++queries;
           }
         }
       }
@@ -444,87 +457,104 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       drain_ring(kv_full(0), C::kStages, issued);
     }
     __syncwarp();
-  } else if (warp == kWarpMma) {
+  } else if (warp == kWarpMma0 || warp == kWarpMma1) {
     // ---------------------------------------------------------------- MMA
+    // One warp per row tile, so that neither tile's chain waits behind the other's in program order.  Few waits and
+    // little code: this warp's instructions are evicted from the cache by the softmax warps' between its turns.
     constexpr uint32_t idesc_qk = f16_idesc<T>(kRows, kKeys, false);
     constexpr uint32_t idesc_pv = f16_idesc<T>(kRows, D, true);
+    constexpr uint32_t kTileLo = C::kTile >> 4;  // a tile in descriptor units
+    const int tt = warp == kWarpMma0 ? 0 : 1;
     bool ok = true;
-    auto stage_ptr = [&](uint32_t i) { return smem + C::OFF_KV + (i % C::kStages) * C::kTile; };
+    uint32_t lead;
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(lead));
     auto wait_all = [&](uint32_t bar, uint32_t parity, int site) {
-      const bool w = wait_bar(bar, parity, ctl, site);
+      const bool w = wait_bar_short(bar, parity, ctl, site);
       return __all_sync(0xffffffffu, w) != 0;
     };
-    auto wait_kv = [&](uint32_t i, int site) { return wait_all(kv_full(i % C::kStages), (i / C::kStages) & 1, site); };
-    const uint32_t q_lo = desc_lo(smem_u32(smem + C::OFF_Q), 0), k_lo = desc_lo(smem_u32(smem + C::OFF_KV), 0);
-    const uint32_t v_lo = desc_lo(smem_u32(smem + C::OFF_KV), kKeys * 128);
-    auto qk = [&](int tt, uint32_t i) {  // S_tt = Q_tt K^T
-      const uint32_t a = q_lo + uint32_t(tt * (C::kTile >> 4)), b = k_lo + (i % C::kStages) * (C::kTile >> 4);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t off = uint32_t((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4;
-        mma_ss(tmem + uint32_t(tt * kKeys), a + off, kDescHi, b + off, kDescHi, idesc_qk, kk > 0);
-      }
-      commit_elected(s_full(tt));
-    };
-    auto pv = [&](int tt, uint32_t i, bool first) {  // O_tt += P_tt V
-      const uint32_t b = v_lo + (i % C::kStages) * (C::kTile >> 4);
-#pragma unroll
-      for (int kk = 0; kk < kKeys / 16; ++kk)
-        mma_ts(tmem + uint32_t(2 * kKeys + tt * D), tmem + uint32_t(tt * kKeys + kk * 8), b + (uint32_t(kk * 16 * 128) >> 4), kDescHi,
-               idesc_pv, !(first && kk == 0));
-    };
-    uint32_t used = 0, queries = 0, steps[2] = {0, 0};  // ring stages, items with keys, key tiles per row tile
+    const uint32_t q_lo = desc_lo(smem_u32(smem + C::OFF_Q), 0) + tt * kTileLo, k_lo = desc_lo(smem_u32(smem + C::OFF_KV), 0);
+    const uint32_t v_lo = desc_lo(smem_u32(smem + C::OFF_KV), kKeys * 128) + kTileLo;
+    const uint32_t s_tm = tmem + uint32_t(tt * kKeys), o_tm = tmem + uint32_t(C::kColO + tt * D);
+    const uint32_t p_tm = tmem + uint32_t(C::kColP + tt * C::kStepP);
+    // ring cursors of the next S and of the next product (one stage behind), with phase parities
+    uint32_t ck = 0, ck_ph = 0, cv = 0;
+    auto advance = [](uint32_t c) { return c + 1 == uint32_t(C::kStages) ? 0u : c + 1; };
+    uint32_t queries = 0, step = 0;
     Item it;
     while (ok && next_item(&it, 512)) {
-      const int n = it.n, last_tt = it.tiles - 1;
+      const int n = it.n;
       if (n == 0) continue;
-      if (!(ok = wait_kv(used, 503) && wait_all(q_full, queries & 1, 502))) break;
-      ++queries;
-      tc_fence_after();
-      for (int tt = 0; tt < it.tiles; ++tt) qk(tt, used);
-      commit_elected(kv_empty(used % C::kStages));
-      if (n == 1) commit_elected(q_empty);
-      for (int i = 0; i < n && ok; ++i) {
-        const uint32_t iv = used + 2 * i + 1, ik = iv + 1;
-        const bool more = i + 1 < n;
-        if (!(ok = wait_kv(iv, 504))) break;
-        if (!PREFIX) {
-          // value rows past the sequence's last key belong to someone else: 0 * anything finite or not must be 0
-          const int valid = it.kn - (it.lo + i) * kKeys;
-          if (valid < kKeys) {
-            for (int j = valid * 8 + lane; j < kKeys * 8; j += 32)
-#pragma unroll
-              for (int c = 0; c < C::kChunks; ++c)
-                *reinterpret_cast<uint4*>(stage_ptr(iv) + c * (kKeys * 128) + j * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async();
-            __syncwarp();
-          }
+      if (tt >= it.tiles) {  // no row in this tile: pass the stages and the queries on
+        for (int i = 0; i < n && ok; ++i) {
+          if (!(ok = wait_all(kv_full(ck), ck_ph, 503))) break;
+          if (lane == 0) mbar_arrive(kv_empty(ck));
+          ck = advance(ck);
+          ck_ph ^= ck == 0;
         }
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-          if (tt > last_tt) break;
-          if (!(ok = wait_all(p_full(tt), steps[tt] & 1, 505 + tt))) break;
-          ++steps[tt];
-          tc_fence_after();
-          pv(tt, iv, i == 0);
-          if (tt == last_tt) commit_elected(kv_empty(iv % C::kStages));
-          if (!more) commit_elected(o_full(tt));
-          if (more) {
-            if (tt == 0 && !(ok = wait_kv(ik, 507))) break;
-            tc_fence_after();
-            qk(tt, ik);
-            if (tt == last_tt) {
-              commit_elected(kv_empty(ik % C::kStages));
-              if (i + 2 == n) commit_elected(q_empty);
-            }
-          }
-        }
+        cv = ck;
+        if (ok && (ok = wait_all(q_full, queries & 1, 502)) && lane == 0) mbar_arrive(q_empty);
+        __syncwarp();
+        ++queries;
+        continue;
       }
-      used += 2 * uint32_t(n);
+      // S = Q K^T for step i + 1, once S is free: read by its softmax (D = 64), or behind the P V that read P from it
+      // (issue order, D = 128)
+      auto next_s = [&](int i) {
+        if (i + 1 >= n) return true;
+        if (!wait_all(kv_full(ck), ck_ph, 503)) return false;
+        if (i < 0 && !wait_all(q_full, queries & 1, 502)) return false;
+        if (C::kOwnP && step + (i >= 0) > 0 && !wait_all(s_free(tt), (step + (i >= 0) + 1) & 1, 514)) return false;
+        tc_fence_after();
+        const uint32_t b = k_lo + ck * (2 * kTileLo);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = uint32_t((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4;
+          mma_ss(lead, s_tm, q_lo + off, b + off, kDescHi, idesc_qk, kk > 0);
+        }
+        commit_lead(lead, s_full(tt));
+        if (i + 2 == n) commit_lead(lead, q_empty);
+        ck = advance(ck);
+        ck_ph ^= ck == 0;
+        return true;
+      };
+      auto product = [&](int i) {  // O += P V of step i
+        if (i < 0) return true;
+        // value rows past the sequence's last key belong to someone else: 0 * anything finite or not must be 0
+        // (both MMA warps write these zeros)
+        const int valid = it.kn - (it.lo + i) * kKeys;
+        if (!PREFIX && valid < kKeys) {
+          unsigned char* v = smem + C::OFF_KV + (2 * cv + 1) * C::kTile;
+#pragma unroll 1
+          for (int j = valid * 8 + lane; j < kKeys * 8; j += 32)
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c)
+              *reinterpret_cast<uint4*>(v + c * (kKeys * 128) + j * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async();
+          __syncwarp();
+        }
+        if (!wait_all(p_full(tt), step & 1, 505)) return false;
+        tc_fence_after();
+        const uint32_t b = v_lo + cv * (2 * kTileLo);
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          mma_ts(lead, o_tm, p_tm + uint32_t(kk * 8), b + uint32_t(kk * 16 * 128 >> 4), kDescHi, idesc_pv, kk > 0 || i > 0);
+        commit_lead(lead, o_full(tt));
+        commit_lead(lead, kv_empty(cv));
+        cv = advance(cv);
+        ++step;
+        return true;
+      };
+      // step -1 makes the first S, step i the next one and this step's product
+#pragma unroll 1
+      for (int i = -1; i < n && ok; ++i) {
+        if constexpr (C::kOwnP) ok = next_s(i) && product(i);
+        else ok = product(i) && next_s(i);
+      }
+      ++queries;
     }
     __syncwarp();
     if (__any_sync(0xffffffffu, *abort_flag != 0)) {  // no MMA may still be in flight when TMEM is freed
-      commit_elected(mma_done);
+      commit_lead(lead, mma_done);
       if (lane == 0) drain_wait(mma_done, 0);
       __syncwarp();
     }
@@ -535,9 +565,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const int tok_in = r / G, g = r - tok_in * G;
     const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + lane_base + uint32_t(t * kKeys);
-    const uint32_t o_col = tmem + lane_base + uint32_t(2 * kKeys + t * D);
+    const uint32_t o_col = tmem + lane_base + uint32_t(C::kColO + t * D);
+    const uint32_t p_col = tmem + lane_base + uint32_t(C::kColP + t * C::kStepP);
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
-    uint32_t steps = 0, ends = 0;
+    uint32_t steps = 0;
     Item it;
     while (next_item(&it, 513)) {
       if (t >= it.tiles) continue;  // no row in this tile
@@ -556,7 +587,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       float m = -INFINITY, l = 0.f;  // m: reference maximum (log2 units) of the stored P and O
       bool ok = true;
       for (int i = 0; i < it.n; ++i, ++steps) {
-        ok = wait_bar(s_full(t), steps & 1, ctl, 508);
+        ok = wait_bar_short(s_full(t), steps & 1, ctl, 508);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
         const int kb = (it.lo + i) * kKeys;
@@ -590,7 +621,13 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             m = top;
             l *= f;
           }
-          if (i > 0) {  // S of this tile is issued behind the previous P V: O is complete
+          // O is complete behind the previous P V (D = 128: S of this tile was issued behind it)
+          if (C::kOwnP && i > 0) {
+            ok = wait_bar_short(o_full(t), (steps - 1) & 1, ctl, 516);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            tc_fence_after();
+          }
+          if (i > 0) {
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
               float o[16];
@@ -625,20 +662,24 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
               for (int j = 0; j < 32; ++j) s[j] = (c + j >= ja && c + j <= jb) ? s[j] : -INFINITY;
             }
           };
-          uint32_t pb[32], pa[16];
-          numerators(sb, pb, whole);
-          numerators(sb + 32, pb + 16, whole);
+          uint32_t pk[32];
+          numerators(sb, pk, whole);
+          numerators(sb + 32, pk + 16, whole);
           tmem_wait_ld32(s0);
           float s1[32];
           tmem_ld32(s_col + 32, s1);
+          if (C::kOwnP && i > 0) ok = wait_bar_short(o_full(t), (steps - 1) & 1, ctl, 517);  // the previous P has been read
+          tmem_st32(p_col + 32, pk);
           hide(s0, 0);
-          numerators(s0, pa, whole);
+          numerators(s0, pk, whole);
           tmem_wait_ld32(s1);
-          tmem_st16(s_col, pa);  // P over columns whose scores have been read
+          if (C::kOwnP) {
+            tc_fence_before();
+            mbar_arrive(s_free(t));
+          }
           hide(s1, 32);
-          numerators(s1, pa, whole);
-          tmem_st16(s_col + 16, pa);
-          tmem_st32(s_col + 32, pb);
+          numerators(s1, pk + 16, whole);
+          tmem_st32(p_col, pk);
         };
         if (masked) write_p(std::false_type{});
         else write_p(std::true_type{});
@@ -647,12 +688,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(p_full(t));
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
       }
       // ---- epilogue: the row's output
       if (ok && it.n > 0) {
-        ok = wait_bar(o_full(t), ends & 1, ctl, 509);
+        ok = wait_bar_short(o_full(t), (steps - 1) & 1, ctl, 509);
         ok = __all_sync(0xffffffffu, ok);
-        ++ends;
         tc_fence_after();
       }
       if (!ok) break;
@@ -711,7 +752,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kWarpMma)
+  if (warp == kWarpMma0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 
