@@ -34,16 +34,40 @@ using namespace tc;
 
 namespace {
 
+// try_wait that lets the hardware hold the warp for up to `ns`, so that waiting warps leave the issue slots to the others
+__device__ __forceinline__ bool mbar_try_wait_ns(uint32_t bar, uint32_t parity, uint32_t ns) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(ns)
+      : "memory");
+  return ok != 0;
+}
+
 // wait_bar with everything but the first try out of line (the waits are many, and code size costs here)
-__device__ __noinline__ bool wait_bar_long(uint32_t bar, uint32_t parity, const Ctl& c, int site) { return wait_bar(bar, parity, c, site); }
+__device__ __noinline__ bool wait_bar_long(uint32_t bar, uint32_t parity, const Ctl& c, int site) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait_ns(bar, parity, 20000)) {
+    if (*c.abort) return false;
+    if (clock64() - t0 > kWaitCycles) {
+      *c.abort = 1;
+      record_fault(c.status, KLC_ERR_DEVICE_TIMEOUT, site, 0);
+      return false;
+    }
+  }
+  return true;
+}
 __device__ __forceinline__ bool wait_bar_short(uint32_t bar, uint32_t parity, const Ctl& c, int site) {
-  return mbar_try_wait(bar, parity) || wait_bar_long(bar, parity, c, site);
+  return mbar_try_wait_ns(bar, parity, 20000) || wait_bar_long(bar, parity, c, site);
 }
 
 constexpr int kRows = 128;     // rows of a row tile (TMEM lanes)
 constexpr int kKeys = 128;     // keys of a key tile
 constexpr int kThreads = 352;  // 8 softmax warps, an MMA warp for each row tile, TMA warp
-constexpr int kWarpMma0 = 8, kWarpTma = 9, kWarpMma1 = 10;
+constexpr int kSoftmaxWarps = 8, kWarpMma0 = 8, kWarpTma = 9, kWarpMma1 = 10;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;
 constexpr int kItems = 2;      // ring of items between the TMA warp and the others
@@ -147,7 +171,7 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
   x.y = fmaxf(x.y, -126.f);
   const float2 t = add2(x, big);
   const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
-  const float2 f = add2(x, make_float2(-n.x, -n.y));
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
   float2 p;
   if constexpr (Elem<T>::kMmaFormat == 1) {
     p = fma2(f, make_float2(0.05517166802f, 0.05517166802f), make_float2(0.24261112211f, 0.24261112211f));
@@ -220,16 +244,19 @@ struct Cfg {
   static constexpr int kChunks = D / 64;                    // 128-byte columns of a head's row
   static constexpr int kTile = kKeys * D * 2;               // bytes of a query, key or value tile
   static constexpr int kStages = D == 64 ? 5 : 2;           // ring of key and value tiles: 160 / 128 KB
-  static constexpr int kFmaPairs = D == 64 ? 3 : 2;         // of 8 pairs of exponentials, on the FMA pipe
+  // of 8 pairs of exponentials, on the FMA pipe: 6016 tokens ran at 643 / 654 / 706 / 690 TFLOP/s with 0 / 1 / 2 / 3
+  // (D = 64), 958 / 970 / 986 / 976 (D = 128)
+  static constexpr int kFmaPairs = 2;
   // TMEM columns: S 0-255, O behind it.  D = 64 leaves room for P, so the next S can be made while this one's
   // exponentials are; with D = 128 P lies over the upper half of S, which is in registers by then.
   static constexpr bool kOwnP = D == 64;
+  static constexpr int kMmaWarps = kOwnP ? 2 : 1;
   static constexpr int kColO = 2 * kKeys;
   static constexpr int kColP = kOwnP ? kColO + 2 * D : kKeys / 2, kStepP = kOwnP ? kKeys / 2 : kKeys;
   static constexpr int OFF_Q = 0;                           // two row tiles
   static constexpr int OFF_KV = 2 * kTile;
   static constexpr int OFF_BAR = OFF_KV + kStages * 2 * kTile;
-  static constexpr int kBars = 2 * kStages + 2 + 8 + 2 * kItems + 1;
+  static constexpr int kBars = 2 * kStages + 2 + 10 + 2 * kItems + 1;
   static constexpr int OFF_MISC = OFF_BAR + kBars * 8;
   static constexpr int OFF_ITEM = OFF_MISC + 16;
   static constexpr int kSmem = OFF_ITEM + kItems * int(sizeof(Item)) + 1024;  // + alignment of the swizzled tiles
@@ -262,9 +289,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   auto p_full = [&](int t) { return bar0 + 8u * (kB + 4 + t); };
   auto o_full = [&](int t) { return bar0 + 8u * (kB + 6 + t); };
   auto s_free = [&](int t) { return bar0 + 8u * (kB + 8 + t); };
-  auto item_full = [&](int i) { return bar0 + 8u * (kB + 10 + i); };
-  auto item_empty = [&](int i) { return bar0 + 8u * (kB + 10 + kItems + i); };
-  const uint32_t mma_done = bar0 + 8u * (kB + 10 + 2 * kItems);
+  auto p_half = [&](int t) { return bar0 + 8u * (kB + 10 + t); };
+  auto item_full = [&](int i) { return bar0 + 8u * (kB + 12 + i); };
+  auto item_empty = [&](int i) { return bar0 + 8u * (kB + 12 + kItems + i); };
+  const uint32_t mma_done = bar0 + 8u * (kB + 12 + 2 * kItems);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
   Item* items = reinterpret_cast<Item*>(smem + C::OFF_ITEM);
@@ -273,21 +301,22 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   if (tid == 32 * kWarpTma) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(kv_full(s), 1);
-      mbar_init(kv_empty(s), 2);  // both MMA warps
+      mbar_init(kv_empty(s), C::kMmaWarps);
     }
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 2);
+    mbar_init(q_empty, C::kMmaWarps);
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full(t), 1);
       mbar_init(p_full(t), kRows);
+      mbar_init(p_half(t), kRows);
       mbar_init(s_free(t), kRows);
       mbar_init(o_full(t), 1);
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(item_full(i), 1);
-      mbar_init(item_empty(i), 10);  // the MMA and the softmax warps
+      mbar_init(item_empty(i), kSoftmaxWarps + C::kMmaWarps);
     }
-    mbar_init(mma_done, 2);
+    mbar_init(mma_done, C::kMmaWarps);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -457,14 +486,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       drain_ring(kv_full(0), C::kStages, issued);
     }
     __syncwarp();
-  } else if (warp == kWarpMma0 || warp == kWarpMma1) {
+  } else if (warp == kWarpMma0 || (warp == kWarpMma1 && C::kMmaWarps == 2)) {
     // ---------------------------------------------------------------- MMA
-    // One warp per row tile, so that neither tile's chain waits behind the other's in program order.  Few waits and
-    // little code: this warp's instructions are evicted from the cache by the softmax warps' between its turns.
+    // D = 64: one warp per row tile, so that neither tile's chain waits behind the other's in program order.  D = 128: one
+    // warp for both, in turns: a tile's P V and next S run as one block of the tensor pipe while the other tile is in its
+    // softmax (issued side by side, the two tiles fell into step and tensor pipe and softmax idled in turns: 812 against 1025
+    // TFLOP/s).  Little code: this warp's instructions are evicted from the cache by the softmax warps' between its turns.
     constexpr uint32_t idesc_qk = f16_idesc<T>(kRows, kKeys, false);
     constexpr uint32_t idesc_pv = f16_idesc<T>(kRows, D, true);
     constexpr uint32_t kTileLo = C::kTile >> 4;  // a tile in descriptor units
-    const int tt = warp == kWarpMma0 ? 0 : 1;
+    constexpr int kMine = 3 - C::kMmaWarps;      // row tiles of this warp
+    const int t0 = warp == kWarpMma0 ? 0 : 1;
     bool ok = true;
     uint32_t lead;
     asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(lead));
@@ -472,19 +504,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       const bool w = wait_bar_short(bar, parity, ctl, site);
       return __all_sync(0xffffffffu, w) != 0;
     };
-    const uint32_t q_lo = desc_lo(smem_u32(smem + C::OFF_Q), 0) + tt * kTileLo, k_lo = desc_lo(smem_u32(smem + C::OFF_KV), 0);
+    const uint32_t q_lo = desc_lo(smem_u32(smem + C::OFF_Q), 0), k_lo = desc_lo(smem_u32(smem + C::OFF_KV), 0);
     const uint32_t v_lo = desc_lo(smem_u32(smem + C::OFF_KV), kKeys * 128) + kTileLo;
-    const uint32_t s_tm = tmem + uint32_t(tt * kKeys), o_tm = tmem + uint32_t(C::kColO + tt * D);
-    const uint32_t p_tm = tmem + uint32_t(C::kColP + tt * C::kStepP);
     // ring cursors of the next S and of the next product (one stage behind), with phase parities
     uint32_t ck = 0, ck_ph = 0, cv = 0;
     auto advance = [](uint32_t c) { return c + 1 == uint32_t(C::kStages) ? 0u : c + 1; };
-    uint32_t queries = 0, step = 0;
+    uint32_t queries = 0, step[2] = {0, 0};
     Item it;
     while (ok && next_item(&it, 512)) {
-      const int n = it.n;
+      const int n = it.n, mine = min(kMine, it.tiles - t0);
       if (n == 0) continue;
-      if (tt >= it.tiles) {  // no row in this tile: pass the stages and the queries on
+      if (mine <= 0) {  // no row in this warp's tile: pass the stages and the queries on
         for (int i = 0; i < n && ok; ++i) {
           if (!(ok = wait_all(kv_full(ck), ck_ph, 503))) break;
           if (lane == 0) mbar_arrive(kv_empty(ck));
@@ -497,58 +527,78 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         ++queries;
         continue;
       }
-      // S = Q K^T for step i + 1, once S is free: read by its softmax (D = 64), or behind the P V that read P from it
-      // (issue order, D = 128)
-      auto next_s = [&](int i) {
+      // S = Q K^T for step i + 1 of this warp's j-th row tile, once S is free: read by its softmax (D = 64), or behind the
+      // P V that read P from it (issue order, D = 128)
+      auto next_s = [&](int i, int j) {
         if (i + 1 >= n) return true;
-        if (!wait_all(kv_full(ck), ck_ph, 503)) return false;
-        if (i < 0 && !wait_all(q_full, queries & 1, 502)) return false;
-        if (C::kOwnP && step + (i >= 0) > 0 && !wait_all(s_free(tt), (step + (i >= 0) + 1) & 1, 514)) return false;
+        const int tt = t0 + j;
+        if (j == 0 && !wait_all(kv_full(ck), ck_ph, 503)) return false;
+        if (j == 0 && i < 0 && !wait_all(q_full, queries & 1, 502)) return false;
+        if (C::kOwnP && step[j] + (i >= 0) > 0 && !wait_all(s_free(tt), (step[j] + (i >= 0) + 1) & 1, 514)) return false;
         tc_fence_after();
-        const uint32_t b = k_lo + ck * (2 * kTileLo);
+        const uint32_t a = q_lo + uint32_t(tt) * kTileLo, b = k_lo + ck * (2 * kTileLo);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = uint32_t((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4;
-          mma_ss(lead, s_tm, q_lo + off, b + off, kDescHi, idesc_qk, kk > 0);
+          mma_ss(lead, tmem + uint32_t(tt * kKeys), a + off, b + off, kDescHi, idesc_qk, kk > 0);
         }
         commit_lead(lead, s_full(tt));
-        if (i + 2 == n) commit_lead(lead, q_empty);
-        ck = advance(ck);
-        ck_ph ^= ck == 0;
+        if (j + 1 == mine) {
+          if (i + 2 == n) commit_lead(lead, q_empty);
+          ck = advance(ck);
+          ck_ph ^= ck == 0;
+        }
         return true;
       };
-      auto product = [&](int i) {  // O += P V of step i
+      auto product = [&](int i, int j) {  // O += P V of step i
         if (i < 0) return true;
+        const int tt = t0 + j;
         // value rows past the sequence's last key belong to someone else: 0 * anything finite or not must be 0
-        // (both MMA warps write these zeros)
+        // (with two MMA warps both write these zeros)
         const int valid = it.kn - (it.lo + i) * kKeys;
-        if (!PREFIX && valid < kKeys) {
+        if (!PREFIX && j == 0 && valid < kKeys) {
           unsigned char* v = smem + C::OFF_KV + (2 * cv + 1) * C::kTile;
 #pragma unroll 1
-          for (int j = valid * 8 + lane; j < kKeys * 8; j += 32)
+          for (int e = valid * 8 + lane; e < kKeys * 8; e += 32)
 #pragma unroll
             for (int c = 0; c < C::kChunks; ++c)
-              *reinterpret_cast<uint4*>(v + c * (kKeys * 128) + j * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(v + c * (kKeys * 128) + e * 16) = make_uint4(0, 0, 0, 0);
           fence_proxy_async();
           __syncwarp();
         }
-        if (!wait_all(p_full(tt), step & 1, 505)) return false;
-        tc_fence_after();
         const uint32_t b = v_lo + cv * (2 * kTileLo);
+        auto keys64 = [&](int k0, bool first) {
 #pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)
-          mma_ts(lead, o_tm, p_tm + uint32_t(kk * 8), b + uint32_t(kk * 16 * 128 >> 4), kDescHi, idesc_pv, kk > 0 || i > 0);
+          for (int kk = k0; kk < k0 + kKeys / 32; ++kk)
+            mma_ts(lead, tmem + uint32_t(C::kColO + tt * D), tmem + uint32_t(C::kColP + tt * C::kStepP + kk * 8),
+                   b + uint32_t(kk * 16 * 128 >> 4), kDescHi, idesc_pv, kk > k0 || !first);
+        };
+        if (!C::kOwnP) {  // P comes in two halves, keys 64-127 first
+          if (!wait_all(p_half(tt), step[j] & 1, 515)) return false;
+          tc_fence_after();
+          keys64(4, i == 0);
+        }
+        if (!wait_all(p_full(tt), step[j] & 1, 505)) return false;
+        tc_fence_after();
+        if (C::kOwnP) keys64(4, i == 0);
+        keys64(0, false);
         commit_lead(lead, o_full(tt));
-        commit_lead(lead, kv_empty(cv));
-        cv = advance(cv);
-        ++step;
+        if (j + 1 == mine) {
+          commit_lead(lead, kv_empty(cv));
+          cv = advance(cv);
+        }
+        ++step[j];
         return true;
       };
       // step -1 makes the first S, step i the next one and this step's product
 #pragma unroll 1
       for (int i = -1; i < n && ok; ++i) {
-        if constexpr (C::kOwnP) ok = next_s(i) && product(i);
-        else ok = product(i) && next_s(i);
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+          if (!ok || j >= mine) break;
+          if constexpr (C::kOwnP) ok = next_s(i, j) && product(i, j);
+          else ok = product(i, j) && next_s(i, j);
+        }
       }
       ++queries;
     }
@@ -558,7 +608,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       if (lane == 0) drain_wait(mma_done, 0);
       __syncwarp();
     }
-  } else {
+  } else if (warp < kSoftmaxWarps) {
     // ---------------------------------------------------------------- softmax
     const int t = warp >> 2;  // row tile
     const int r = tid & (kRows - 1);
@@ -662,24 +712,43 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
               for (int j = 0; j < 32; ++j) s[j] = (c + j >= ja && c + j <= jb) ? s[j] : -INFINITY;
             }
           };
-          uint32_t pk[32];
-          numerators(sb, pk, whole);
-          numerators(sb + 32, pk + 16, whole);
-          tmem_wait_ld32(s0);
-          float s1[32];
-          tmem_ld32(s_col + 32, s1);
-          if (C::kOwnP && i > 0) ok = wait_bar_short(o_full(t), (steps - 1) & 1, ctl, 517);  // the previous P has been read
-          tmem_st32(p_col + 32, pk);
-          hide(s0, 0);
-          numerators(s0, pk, whole);
-          tmem_wait_ld32(s1);
-          if (C::kOwnP) {
+          if constexpr (C::kOwnP) {
+            uint32_t pk[32];
+            numerators(sb, pk, whole);
+            numerators(sb + 32, pk + 16, whole);
+            tmem_wait_ld32(s0);
+            float s1[32];
+            tmem_ld32(s_col + 32, s1);
+            if (i > 0) ok = wait_bar_short(o_full(t), (steps - 1) & 1, ctl, 517);  // the previous P V still reads P till then
+            tmem_st32(p_col + 32, pk);
+            hide(s0, 0);
+            numerators(s0, pk, whole);
+            tmem_wait_ld32(s1);
             tc_fence_before();
             mbar_arrive(s_free(t));
+            hide(s1, 32);
+            numerators(s1, pk + 16, whole);
+            tmem_st32(p_col, pk);
+          } else {
+            uint32_t pk[16];
+            numerators(sb, pk, whole);
+            tmem_st16(p_col + 32, pk);
+            tmem_wait_ld32(s0);
+            numerators(sb + 32, pk, whole);
+            tmem_st16(p_col + 48, pk);
+            float s1[32];
+            tmem_ld32(s_col + 32, s1);
+            tmem_wait_st();  // keys 64-127: their half of the product starts here
+            tc_fence_before();
+            mbar_arrive(p_half(t));
+            hide(s0, 0);
+            numerators(s0, pk, whole);
+            tmem_st16(p_col, pk);
+            tmem_wait_ld32(s1);
+            hide(s1, 32);
+            numerators(s1, pk, whole);
+            tmem_st16(p_col + 16, pk);
           }
-          hide(s1, 32);
-          numerators(s1, pk + 16, whole);
-          tmem_st32(p_col, pk);
         };
         if (masked) write_p(std::false_type{});
         else write_p(std::true_type{});
