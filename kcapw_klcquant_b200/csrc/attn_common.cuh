@@ -14,7 +14,7 @@ namespace attn {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kMaxBatch = 4096;  // sequences per decode call (the kernels keep one prefix sum per sequence)
+constexpr int kMaxBatch = 4096;  // sequences per decode call (each CTA keeps 16 bytes of plan per sequence)
 
 template <typename T>
 struct Elem;

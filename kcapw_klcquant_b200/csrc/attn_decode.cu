@@ -5,14 +5,14 @@
 // it, about G flops a byte: HBM bound, so the kernel is built around keeping
 // loads in flight and every SM busy whatever the lengths are.
 //
-//   * The work is one list of 64-key tiles over (sequence, key head, tile of
+//   * The work is one list of key tiles (128 keys of width 64, 64 of width 128: 32 KB) over (sequence, key head, tile of
 //     16 query heads); CTA c of N takes an equal contiguous range of it.  A
 //     range that cuts an item leaves a share (m, l, o) of it in the workspace, at
 //     most two per CTA, and a second kernel joins the shares.  The split needs
 //     only the lengths, which stay on the device: no host sync, and a captured step serves growing
 //     lengths.
-//   * Per CTA one TMA warp walks the page table (ids prefetched 32 at a time) and fills a ring of 64-key
-//     tiles; four warps take 16 keys each of a tile (mma.sync m16n8k16: a row
+//   * Per CTA one TMA warp walks the page table (ids prefetched 32 at a time) and fills a ring of
+//     tiles; four warps take a quarter of its keys each (mma.sync m16n8k16: a row
 //     tile is 16 heads, far too few to feed tcgen05's 128 rows, and the tensor rate
 //     is not the bound).  Each warp keeps its own running
 //     maximum, sum and 16 x D output; the four are joined once per item.
@@ -33,30 +33,31 @@ using namespace tc;
 
 namespace {
 
-constexpr int kTileKeys = 64;
 constexpr int kThreads = 160;  // four math warps, one TMA warp
 constexpr int kCtasPerSm = 2;
 constexpr int kRowTile = 16;
 
+// A sequence in a CTA's plan: key tiles of the sequences before it, and the keys [klo, len) its own pages contribute.
+struct Seq {
+  int cum, klo, len, prefix;
+};
+
 template <int D>
 struct DCfg {
+  static constexpr int kTileKeys = D == 64 ? 128 : 64;        // 32 KB of keys and values either way
+  static constexpr int kGroups = kTileKeys / 64;              // groups of 16 keys a warp takes of a tile
   static constexpr int kChunks = D / 64;
   static constexpr int kHalf = kTileKeys * D * 2;             // bytes of a key (or value) tile
   static constexpr int kStage = 2 * kHalf;                    // keys and values
-  static constexpr int kStages = D == 64 ? 5 : 3;             // 80 / 96 KB in flight per CTA
+  static constexpr int kStages = 3;                           // 96 KB in flight per CTA
   static constexpr int kOld = D + 8;                          // row pitch of the join buffer (floats)
   static constexpr int OFF_RING = 0;
   static constexpr int OFF_O = kStages * kStage;              // [16][kOld] fp32
   static constexpr int OFF_ML = OFF_O + kRowTile * kOld * 4;  // [4][16] (m, l)
   static constexpr int OFF_BAR = OFF_ML + 4 * kRowTile * 8;
   static constexpr int OFF_MISC = OFF_BAR + 2 * kStages * 8;
-  static constexpr int OFF_CUM = OFF_MISC + 64;               // [batch + 1] tiles before each sequence
-  static size_t smem(int64_t batch) { return size_t(OFF_CUM) + size_t(batch + 1) * 4 + 1024; }
-};
-
-// The keys [klo, len) a sequence's own pages contribute, as a first tile and a number of tiles.
-struct Span {
-  int klo, len, tile0, tiles;
+  static constexpr int OFF_SEQ = OFF_MISC + 64;               // [batch + 1] Seq
+  static size_t smem(int64_t batch) { return size_t(OFF_SEQ) + size_t(batch + 1) * sizeof(Seq) + 1024; }
 };
 
 __device__ __forceinline__ int prefix_of(const DecodeParams& p, int b) {
@@ -72,18 +73,22 @@ __device__ __forceinline__ int prefix_of(const DecodeParams& p, int b) {
   return pre < 0 || pre % p.page_size != 0 || pre > p.table_width * p.page_size ? 0 : pre;  // reported by the prefix kernel
 }
 
-__device__ __forceinline__ Span span_of(const DecodeParams& p, int b, bool report) {
+__device__ __forceinline__ Seq seq_of(const DecodeParams& p, int b, bool report) {
   int len = p.lens[b];
   if (len < 0 || int64_t(len) > int64_t(p.table_width) * p.page_size) {
     if (report) record_fault(p.status, KLC_ERR_DEVICE_FAULT, 510, b);
     len = 0;
   }
-  Span s;
+  Seq s;
+  s.cum = 0;
+  s.prefix = prefix_of(p, b);
+  s.klo = max(p.window > 0 ? max(0, len - p.window) : 0, s.prefix);
   s.len = len;
-  s.klo = max(p.window > 0 ? max(0, len - p.window) : 0, prefix_of(p, b));
-  s.tile0 = s.klo / kTileKeys;
-  s.tiles = len > s.klo ? (len + kTileKeys - 1) / kTileKeys - s.tile0 : 0;
   return s;
+}
+template <int TK>
+__device__ __forceinline__ int tiles_of(const Seq& s) {
+  return s.len > s.klo ? (s.len + TK - 1) / TK - s.klo / TK : 0;
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -131,19 +136,20 @@ struct Run {
   int tiles;          // of the whole item
 };
 
-__device__ __forceinline__ Run run_at(const int* cum, int batch, int hrs, int64_t x, int64_t end) {
+__device__ __forceinline__ Run run_at(const Seq* seqs, int batch, int hrs, int64_t x, int64_t end) {
   int lo = 0, hi = batch;  // last sequence with cum * hrs <= x (its count is positive, since x is inside)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (int64_t(cum[mid]) * hrs <= x) lo = mid;
+    if (int64_t(seqs[mid].cum) * hrs <= x) lo = mid;
     else hi = mid;
   }
   Run r;
   r.b = lo;
-  r.tiles = cum[lo + 1] - cum[lo];
-  const int64_t rel = x - int64_t(cum[lo]) * hrs;
-  r.hr = int(rel / r.tiles);
-  r.tile = int(rel - int64_t(r.hr) * r.tiles);
+  const int cum = seqs[lo].cum;
+  r.tiles = seqs[lo + 1].cum - cum;
+  const uint32_t rel = uint32_t(x - int64_t(cum) * hrs);  // tiles * hrs of one sequence: fits (checked by the host)
+  r.hr = int(rel / uint32_t(r.tiles));
+  r.tile = int(rel - uint32_t(r.hr) * uint32_t(r.tiles));
   r.n = int(min(int64_t(r.tiles - r.tile), end - x));
   return r;
 }
@@ -155,7 +161,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int* cum = reinterpret_cast<int*>(smem + C::OFF_CUM);
+  constexpr int TK = C::kTileKeys;
+  Seq* seqs = reinterpret_cast<Seq*>(smem + C::OFF_SEQ);
   int* scan_s = reinterpret_cast<int*>(smem + C::OFF_MISC + 16);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC);
   const Ctl ctl{abort_flag, p.status};
@@ -177,7 +184,10 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   // ---- prefix sums of the sequences' tiles
   const int per = (p.batch + kThreads - 1) / kThreads, b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
   int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += span_of(p, b, blockIdx.x == 0).tiles;
+  for (int b = b0; b < b1; ++b) {
+    seqs[b] = seq_of(p, b, blockIdx.x == 0);
+    mine += tiles_of<TK>(seqs[b]);
+  }
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -189,36 +199,37 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   int at = incl - mine;
   for (int w = 0; w < warp; ++w) at += scan_s[w];
   for (int b = b0; b < b1; ++b) {
-    cum[b] = at;
+    seqs[b].cum = at;
     if (blockIdx.x == 0) p.cum[b] = at;
-    at += span_of(p, b, false).tiles;
+    at += tiles_of<TK>(seqs[b]);
     if (b == p.batch - 1) {
-      cum[p.batch] = at;
+      seqs[p.batch].cum = at;
       if (blockIdx.x == 0) p.cum[p.batch] = at;
     }
   }
   __syncthreads();
   const int hrs = p.kv_heads * p.row_tiles;
-  const int64_t total = int64_t(cum[p.batch]) * hrs;
+  const int64_t total = int64_t(seqs[p.batch].cum) * hrs;
   const int64_t nc = min(int64_t(gridDim.x), total);  // CTAs with work: at least one tile each
   const int64_t x0 = blockIdx.x < nc ? total * blockIdx.x / nc : 0, x1 = blockIdx.x < nc ? total * (blockIdx.x + 1) / nc : 0;
 
   if (warp == 4) {
     // ---------------------------------------------------------------- loads
-    const int box = min(p.page_size, kTileKeys), parts = kTileKeys / box;
+    const int box = min(p.page_size, TK), parts = TK / box;
     const int boxes = parts * C::kChunks * 2;  // at most 16: lane j issues box j
     const int bkv = lane / (parts * C::kChunks), bc = (lane / parts) % C::kChunks, bp = lane % parts;
     uint32_t issued = 0;
     bool ok = true;
     for (int64_t x = x0; x < x1 && ok;) {
-      const Run r = run_at(cum, p.batch, hrs, x, x1);
-      const Span sp = span_of(p, r.b, false);
+      const Run r = run_at(seqs, p.batch, hrs, x, x1);
+      const Seq sp = seqs[r.b];
+      const int tile0 = sp.klo / TK;
       const int kvh = r.hr / p.row_tiles;
       const int32_t* table = p.block_table + int64_t(r.b) * p.table_stride;
       int have = -1, cached = 0;  // lane's page id of table entry have + lane
       for (int i = 0; i < r.n && ok; ++i, ++issued) {
-        const int key0 = (sp.tile0 + r.tile + i) * kTileKeys;
-        const int e0 = key0 / p.page_size, e1 = (key0 + kTileKeys - 1) / p.page_size;
+        const int key0 = (tile0 + r.tile + i) * TK;
+        const int e0 = key0 / p.page_size, e1 = (key0 + TK - 1) / p.page_size;
         if (have < 0 || e1 >= have + 32) {
           have = e0;
           const int e = have + lane;
@@ -238,7 +249,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         if (lane == 0) mbar_arrive_expect_tx(full(s), uint32_t(C::kStage));
         __syncwarp();
         if (lane < boxes)
-          tma_load_4d(smem_u32(smem + C::OFF_RING + s * C::kStage + bkv * C::kHalf + bc * (kTileKeys * 128) + bp * box * 128),
+          tma_load_4d(smem_u32(smem + C::OFF_RING + s * C::kStage + bkv * C::kHalf + bc * (TK * 128) + bp * box * 128),
                       bkv ? &map_v : &map_k, bc * 64, key % p.page_size, kvh, page, full(s));
       }
       x += r.n;
@@ -252,8 +263,9 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     uint32_t used = 0;
     bool ok = true;
     for (int64_t x = x0; x < x1 && ok;) {
-      const Run r = run_at(cum, p.batch, hrs, x, x1);
-      const Span sp = span_of(p, r.b, false);
+      const Run r = run_at(seqs, p.batch, hrs, x, x1);
+      const Seq sp = seqs[r.b];
+      const int tile0 = sp.klo / TK;
       const int kvh = r.hr / p.row_tiles, rt = r.hr - kvh * p.row_tiles;
       const int rows = min(kRowTile, G - rt * kRowTile);
       const int head0 = kvh * G + rt * kRowTile;
@@ -278,23 +290,30 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         ok = wait_bar(full(s), (used / C::kStages) & 1, ctl, 513);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         const uint32_t kbase = smem_u32(smem + C::OFF_RING + s * C::kStage), vbase = kbase + C::kHalf;
-        // S = Q K^T for this warp's 16 keys: two groups of eight
-        float sc[2][4] = {};
-        const int krow = warp * 16 + ((lane >> 4) << 3) + (lane & 7);
+        // S = Q K^T for this warp's kGroups x 16 keys
+        constexpr int NG = C::kGroups;
+        float sc[2 * NG][4] = {};
+        const int wkey = warp * (16 * NG);  // the warp's first key in the tile
+        const int krow = wkey + ((lane >> 4) << 3) + (lane & 7);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const int ch = (kk * 2 + ((lane >> 3) & 1)) & 7;
-          uint32_t kf[4];
-          ldsm4(kbase + (kk >> 2) * (kTileKeys * 128) + krow * 128 + ((ch ^ (krow & 7)) << 4), kf);
-          mma16816<T>(sc[0], qf[kk], kf[0], kf[1]);
-          mma16816<T>(sc[1], qf[kk], kf[2], kf[3]);
+#pragma unroll
+          for (int gk = 0; gk < NG; ++gk) {
+            uint32_t kf[4];
+            ldsm4(kbase + (kk >> 2) * (TK * 128) + (krow + 16 * gk) * 128 + ((ch ^ (krow & 7)) << 4), kf);
+            mma16816<T>(sc[2 * gk], qf[kk], kf[0], kf[1]);
+            mma16816<T>(sc[2 * gk + 1], qf[kk], kf[2], kf[3]);
+          }
         }
-        const int key = (sp.tile0 + r.tile + i) * kTileKeys + warp * 16;  // of the warp's first
-        uint32_t vmask[2] = {0xffffffffu, 0xffffffffu};
-        if (key < sp.klo || key + 16 > sp.len) {
+        const int key = (tile0 + r.tile + i) * TK + wkey;
+        uint32_t vmask[2 * NG];
+#pragma unroll
+        for (int h = 0; h < 2 * NG; ++h) vmask[h] = 0xffffffffu;
+        if (key < sp.klo || key + 16 * NG > sp.len) {
           // hidden keys: no weight, and a value row of zeros (what is stored there may not be a number)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2 * NG; ++h)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int kx = key + h * 8 + quad * 2 + e;
@@ -304,10 +323,12 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
               }
             }
         }
-        uint32_t pf[4];
+        uint32_t pf[NG][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // rows `row` and `row + 8`
-          float mx = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
+          float mx = sc[0][2 * h];
+#pragma unroll
+          for (int c = 0; c < 2 * NG; ++c) mx = fmaxf(mx, fmaxf(sc[c][2 * h], sc[c][2 * h + 1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * p.scale_log2;
           if (mx > m[h]) {
@@ -321,22 +342,28 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             }
           }
           const float ref = m[h] == -INFINITY ? 0.f : m[h];
-          float e[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) e[c] = exp2_approx(fmaf(sc[c >> 1][2 * h + (c & 1)], p.scale_log2, -ref));
-          l[h] += (e[0] + e[1]) + (e[2] + e[3]);  // this lane's keys; summed over the quad at the end
-          pf[h] = Elem<T>::pack(e[0], e[1]);
-          pf[2 + h] = Elem<T>::pack(e[2], e[3]);
+          for (int gk = 0; gk < NG; ++gk) {
+            float e[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) e[c] = exp2_approx(fmaf(sc[2 * gk + (c >> 1)][2 * h + (c & 1)], p.scale_log2, -ref));
+            l[h] += (e[0] + e[1]) + (e[2] + e[3]);  // this lane's keys; summed over the quad at the end
+            pf[gk][h] = Elem<T>::pack(e[0], e[1]);
+            pf[gk][2 + h] = Elem<T>::pack(e[2], e[3]);
+          }
         }
         // O += P V
-        const int vrow = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+        const int vrow = wkey + (((lane >> 3) & 1) << 3) + (lane & 7);
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
           const int ch = (j * 2 + (lane >> 4)) & 7;
-          uint32_t vf[4];
-          ldsm4_t(vbase + (j >> 2) * (kTileKeys * 128) + vrow * 128 + ((ch ^ (vrow & 7)) << 4), vf);
-          mma16816<T>(o[2 * j], pf, vf[0] & vmask[0], vf[1] & vmask[1]);
-          mma16816<T>(o[2 * j + 1], pf, vf[2] & vmask[0], vf[3] & vmask[1]);
+#pragma unroll
+          for (int gk = 0; gk < NG; ++gk) {
+            uint32_t vf[4];
+            ldsm4_t(vbase + (j >> 2) * (TK * 128) + (vrow + 16 * gk) * 128 + ((ch ^ (vrow & 7)) << 4), vf);
+            mma16816<T>(o[2 * j], pf[gk], vf[0] & vmask[2 * gk], vf[1] & vmask[2 * gk + 1]);
+            mma16816<T>(o[2 * j + 1], pf[gk], vf[2] & vmask[2 * gk], vf[3] & vmask[2 * gk + 1]);
+          }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(s));
@@ -377,7 +404,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         math_sync();
       }
       // ---- out: the finished row, or the CTA's share of a cut one
-      const bool cut = r.n != r.tiles, whole = !cut && prefix_of(p, r.b) == 0;
+      const bool cut = r.n != r.tiles, whole = !cut && sp.prefix == 0;
       const int slot = 2 * blockIdx.x + (x > x0 ? 1 : 0);
       constexpr int kPerRow = D / 8;  // eight values a thread
       for (int idx = tid; idx < rows * kPerRow; idx += 128) {
@@ -595,7 +622,8 @@ extern "C" int klc_attn_decode(const klc_attn_dims* dims, const void* q, int64_t
   KLC_CHECK_ARG(page_size_ok(page_size), "klc_attn_decode: page_size must be 16, 32, 64 or 128");
   KLC_CHECK_ARG(pages >= 1 && pages < (1 << 30), "klc_attn_decode: pages must be between 1 and 2^30");
   KLC_CHECK_ARG(table_width >= 0 && table_width < (int64_t(1) << 31) && table_stride >= table_width, "klc_attn_decode: bad block table width or stride");
-  KLC_CHECK_ARG(table_width * page_size < (int64_t(1) << 31) && batch * (table_width * page_size / kTileKeys + 1) < (int64_t(1) << 31),
+  KLC_CHECK_ARG(table_width * page_size < (int64_t(1) << 31) && batch * (table_width * page_size / 64 + 1) < (int64_t(1) << 31) &&
+                    int64_t(dims->heads) * (table_width * page_size / 64 + 1) < (int64_t(1) << 31),
                 "klc_attn_decode: the block table covers too many keys");
   if (batch == 0) return KLC_OK;
   const int d = dims->head_dim;
@@ -654,7 +682,7 @@ extern "C" int klc_attn_decode(const klc_attn_dims* dims, const void* q, int64_t
     p.after_prefix = pdl_enabled();
   }
   CUtensorMap mk, mv;
-  const int box = std::min(page_size, kTileKeys);
+  const int box = std::min(page_size, d == 64 ? DCfg<64>::kTileKeys : DCfg<128>::kTileKeys);
   if ((st = pool_map(&mk, dims->dtype, d, k_pages, pages, dims->kv_heads, page_size, page_stride, box)) != KLC_OK) return st;
   if ((st = pool_map(&mv, dims->dtype, d, v_pages, pages, dims->kv_heads, page_size, page_stride, box)) != KLC_OK) return st;
   if (dims->dtype == KLC_BF16)
