@@ -36,8 +36,11 @@ namespace {
 constexpr int kThreads = 160;  // four math warps, one TMA warp
 constexpr int kCtasPerSm = 2;
 constexpr int kRowTile = 16;
+// What starting and ending an item costs a CTA, in tiles (queries, joining the warps, the output): counted into the split, or
+// CTAs that get many short sequences finish last (32 sequences of 100 to 9000 keys: 60 / 51 / 46 / 44 / 43 us with 0 / 1 / 2 / 3 / 4).
+constexpr int kItemCost = 3;
 
-// A sequence in a CTA's plan: key tiles of the sequences before it, and the keys [klo, len) its own pages contribute.
+// A sequence in a CTA's plan: units (tiles, and kItemCost per item) of the sequences before it over one key head and row tile, and the keys [klo, len) its own pages contribute.
 struct Seq {
   int cum, klo, len, prefix;
 };
@@ -87,8 +90,8 @@ __device__ __forceinline__ Seq seq_of(const DecodeParams& p, int b, bool report)
   return s;
 }
 template <int TK>
-__device__ __forceinline__ int tiles_of(const Seq& s) {
-  return s.len > s.klo ? (s.len + TK - 1) / TK - s.klo / TK : 0;
+__device__ __forceinline__ int units_of(const Seq& s) {
+  return s.len > s.klo ? (s.len + TK - 1) / TK - s.klo / TK + kItemCost : 0;
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -129,9 +132,11 @@ __device__ __forceinline__ bool math_sync_and(bool ok) {
   return all != 0;
 }
 
-// A run of one item's tiles in a CTA's range.
+// A run of one item's units in a CTA's range: kItemCost units, then its tiles.  A run that ends inside the former has no
+// tile (the next CTA takes the item).
 struct Run {
   int b, hr;          // sequence; key head * row tiles + row tile
+  int units;          // of the run
   int tile, n;        // first tile (counted from the item's first) and number of tiles
   int tiles;          // of the whole item
 };
@@ -145,12 +150,14 @@ __device__ __forceinline__ Run run_at(const Seq* seqs, int batch, int hrs, int64
   }
   Run r;
   r.b = lo;
-  const int cum = seqs[lo].cum;
-  r.tiles = seqs[lo + 1].cum - cum;
-  const uint32_t rel = uint32_t(x - int64_t(cum) * hrs);  // tiles * hrs of one sequence: fits (checked by the host)
-  r.hr = int(rel / uint32_t(r.tiles));
-  r.tile = int(rel - uint32_t(r.hr) * uint32_t(r.tiles));
-  r.n = int(min(int64_t(r.tiles - r.tile), end - x));
+  const int cum = seqs[lo].cum, units = seqs[lo + 1].cum - cum;
+  const uint32_t rel = uint32_t(x - int64_t(cum) * hrs);  // units * hrs of one sequence: fits (checked by the host)
+  r.hr = int(rel / uint32_t(units));
+  const int u0 = int(rel - uint32_t(r.hr) * uint32_t(units));
+  r.units = int(min(int64_t(units - u0), end - x));
+  r.tiles = units - kItemCost;
+  r.tile = max(0, u0 - kItemCost);
+  r.n = max(0, u0 + r.units - kItemCost) - r.tile;
   return r;
 }
 
@@ -178,6 +185,10 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (tid == 32 * 4) {
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
+  }
   pdl_trigger();
   if (!p.after_prefix) pdl_wait();  // behind the prefix kernel, its inputs are complete already
 
@@ -186,7 +197,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   int mine = 0;
   for (int b = b0; b < b1; ++b) {
     seqs[b] = seq_of(p, b, blockIdx.x == 0);
-    mine += tiles_of<TK>(seqs[b]);
+    mine += units_of<TK>(seqs[b]);
   }
   int incl = mine;
 #pragma unroll
@@ -201,7 +212,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   for (int b = b0; b < b1; ++b) {
     seqs[b].cum = at;
     if (blockIdx.x == 0) p.cum[b] = at;
-    at += tiles_of<TK>(seqs[b]);
+    at += units_of<TK>(seqs[b]);
     if (b == p.batch - 1) {
       seqs[p.batch].cum = at;
       if (blockIdx.x == 0) p.cum[p.batch] = at;
@@ -210,7 +221,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   __syncthreads();
   const int hrs = p.kv_heads * p.row_tiles;
   const int64_t total = int64_t(seqs[p.batch].cum) * hrs;
-  const int64_t nc = min(int64_t(gridDim.x), total);  // CTAs with work: at least one tile each
+  const int64_t nc = min(int64_t(gridDim.x), total);  // CTAs with a unit at least
   const int64_t x0 = blockIdx.x < nc ? total * blockIdx.x / nc : 0, x1 = blockIdx.x < nc ? total * (blockIdx.x + 1) / nc : 0;
 
   if (warp == 4) {
@@ -252,7 +263,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           tma_load_4d(smem_u32(smem + C::OFF_RING + s * C::kStage + bkv * C::kHalf + bc * (TK * 128) + bp * box * 128),
                       bkv ? &map_v : &map_k, bc * 64, key % p.page_size, kvh, page, full(s));
       }
-      x += r.n;
+      x += r.units;
     }
     if (!ok) drain_ring(full(0), C::kStages, issued);
   } else {
@@ -266,6 +277,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const Run r = run_at(seqs, p.batch, hrs, x, x1);
       const Seq sp = seqs[r.b];
       const int tile0 = sp.klo / TK;
+      if (r.n == 0) break;  // the range ends inside the item's start
       const int kvh = r.hr / p.row_tiles, rt = r.hr - kvh * p.row_tiles;
       const int rows = min(kRowTile, G - rt * kRowTile);
       const int head0 = kvh * G + rt * kRowTile;
@@ -439,7 +451,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
       }
       math_sync();  // the buffers are free for the next item
-      x += r.n;
+      x += r.units;
     }
   }
   if (p.after_prefix) pdl_wait();  // this grid ends after the prefix kernel: the join waits for both
@@ -461,15 +473,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const Decode
   const int b = int(rid / p.heads), head = int(rid - int64_t(b) * p.heads);
   const int kvh = head / p.group, g = head - kvh * p.group, rt = g / kRowTile, rr = g - rt * kRowTile;
   const int hrs = p.kv_heads * p.row_tiles;
-  const int c0 = p.cum[b], tiles = p.cum[b + 1] - c0;
+  const int c0 = p.cum[b], units = p.cum[b + 1] - c0;
   const int64_t total = int64_t(p.cum[p.batch]) * hrs, nc = min(int64_t(ctas), total);
   const bool prefix = prefix_of(p, b) > 0;
   int first = 0, last = -1;  // CTAs that hold shares of the item
   int64_t i0 = 0;
-  if (tiles > 0) {
-    i0 = int64_t(c0) * hrs + int64_t(kvh * p.row_tiles + rt) * tiles;
-    first = int(((i0 + 1) * nc - 1) / total);
-    last = int(((i0 + tiles) * nc - 1) / total);
+  if (units > 0) {  // CTA of a unit u: the last one whose range starts at or before u
+    i0 = int64_t(c0) * hrs + int64_t(kvh * p.row_tiles + rt) * units;
+    first = int(((i0 + kItemCost + 1) * nc - 1) / total);
+    last = int(((i0 + units) * nc - 1) / total);
   }
   if (!prefix && first == last) return;  // written by the decode kernel
 
@@ -622,8 +634,8 @@ extern "C" int klc_attn_decode(const klc_attn_dims* dims, const void* q, int64_t
   KLC_CHECK_ARG(page_size_ok(page_size), "klc_attn_decode: page_size must be 16, 32, 64 or 128");
   KLC_CHECK_ARG(pages >= 1 && pages < (1 << 30), "klc_attn_decode: pages must be between 1 and 2^30");
   KLC_CHECK_ARG(table_width >= 0 && table_width < (int64_t(1) << 31) && table_stride >= table_width, "klc_attn_decode: bad block table width or stride");
-  KLC_CHECK_ARG(table_width * page_size < (int64_t(1) << 31) && batch * (table_width * page_size / 64 + 1) < (int64_t(1) << 31) &&
-                    int64_t(dims->heads) * (table_width * page_size / 64 + 1) < (int64_t(1) << 31),
+  KLC_CHECK_ARG(table_width * page_size < (int64_t(1) << 31) && batch * (table_width * page_size / 64 + 1 + kItemCost) < (int64_t(1) << 31) &&
+                    int64_t(dims->heads) * (table_width * page_size / 64 + 1 + kItemCost) < (int64_t(1) << 31),
                 "klc_attn_decode: the block table covers too many keys");
   if (batch == 0) return KLC_OK;
   const int d = dims->head_dim;

@@ -54,7 +54,7 @@ struct DecodeParams {
   float* lse;
   DeviceStatus* status;
   // workspace
-  int* cum;             // [batch + 1] key tiles before each sequence
+  int* cum;             // [batch + 1] the split's units before each sequence
   float2* part_ml;      // [2 * ctas][16] shares of cut items
   float* part_o;        // [2 * ctas][16][D]
   float2* prefix_ml;    // [splits + 1][batch][heads]: the prefix's shares, and uncut items behind a prefix

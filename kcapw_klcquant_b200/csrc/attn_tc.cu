@@ -299,6 +299,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const Ctl ctl{abort_flag, p.status};
 
   if (tid == 32 * kWarpTma) {
+    prefetch_map(&map_q);
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(kv_full(s), 1);
       mbar_init(kv_empty(s), C::kMmaWarps);
