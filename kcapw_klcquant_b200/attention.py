@@ -23,7 +23,7 @@ import threading
 import torch
 
 from . import _lib
-from .moe import workspace
+from .moe import as_bf16, workspace
 
 _STATUS: dict[int, torch.Tensor] = {}
 _STATUS_LOCK = threading.Lock()
@@ -364,3 +364,73 @@ def rope_append(
             k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], ps, page_stride, block_table.data_ptr(), rows_n, width,
             table_stride, _lib.ptr(device_status(dev)), stream))
     return (o, ko) if return_k else o
+
+
+class AttentionLayer:
+    """The attention half of a decoder layer: q, k and v projections, rotary embedding, attention, output projection.
+
+    ``qkv_weight`` bf16 [(heads + 2 kv_heads) * D, H] holds the q, k and v rows one after the other, ``o_weight`` [H, heads * D];
+    biases and ``sinks`` [heads] may be None.  ``window`` as for :func:`attn_prompt`.  The projections are plain library
+    products (torch.nn.functional.linear).
+    """
+
+    def __init__(self, qkv_weight: torch.Tensor, o_weight: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
+                 qkv_bias: torch.Tensor | None = None, o_bias: torch.Tensor | None = None, sinks: torch.Tensor | None = None,
+                 window: int = 0, scale: float | None = None):
+        rows = (heads + 2 * kv_heads) * head_dim
+        if qkv_weight.dim() != 2 or qkv_weight.shape[0] != rows:
+            raise ValueError(f"qkv_weight must be [{rows}, hidden], got {tuple(qkv_weight.shape)}")
+        if o_weight.shape != (qkv_weight.shape[1], heads * head_dim):
+            raise ValueError(f"o_weight must be [{qkv_weight.shape[1]}, {heads * head_dim}], got {tuple(o_weight.shape)}")
+        if kv_heads < 1 or heads % kv_heads != 0 or head_dim not in (64, 128):
+            raise ValueError("heads must be a multiple of kv_heads, head_dim 64 or 128")
+        dev = qkv_weight.device
+        self.heads, self.kv_heads, self.head_dim, self.window, self.scale = int(heads), int(kv_heads), int(head_dim), int(window), scale
+        self.qkv_weight, self.o_weight = as_bf16(qkv_weight, dev), as_bf16(o_weight, dev)
+        self.qkv_bias = None if qkv_bias is None else as_bf16(qkv_bias, dev)
+        self.o_bias = None if o_bias is None else as_bf16(o_bias, dev)
+        self.sinks = None if sinks is None else sinks.to(device=dev, dtype=torch.float32).contiguous()
+        if self.sinks is not None and self.sinks.shape != (heads,):
+            raise ValueError(f"sinks must be [{heads}]")
+
+    @classmethod
+    def from_tensors(cls, layer_idx: int, tensors: dict[str, torch.Tensor], device, heads: int, kv_heads: int, head_dim: int,
+                     window: int = 0) -> "AttentionLayer":
+        """Build from checkpoint-named tensors (``model.layers.{L}.self_attn.*``; biases and sinks optional)."""
+        p = f"model.layers.{layer_idx}.self_attn"
+        dev = torch.device(device)
+
+        def get(name):
+            t = tensors.get(f"{p}.{name}")
+            return None if t is None else t.to(dev)
+
+        parts = [get(f"{n}_proj.bias") for n in "qkv"]
+        if any(b is None for b in parts) and not all(b is None for b in parts):
+            raise ValueError("q, k and v must all have a bias or none")
+        return cls(torch.cat([get(f"{n}_proj.weight") for n in "qkv"]), get("o_proj.weight"), heads, kv_heads, head_dim,
+                   qkv_bias=None if parts[0] is None else torch.cat(parts), o_bias=get("o_proj.bias"), sinks=get("sinks"), window=window)
+
+    def project(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """q [T, heads, D], k and v [T, kv_heads, D] of x bf16 [T, H]: slices of one product."""
+        h, g = self.heads, self.kv_heads
+        qkv = torch.nn.functional.linear(x, self.qkv_weight, self.qkv_bias).view(x.shape[0], h + 2 * g, self.head_dim)
+        return qkv[:, :h], qkv[:, h:h + g], qkv[:, h + g:]
+
+    def output(self, o: torch.Tensor) -> torch.Tensor:
+        return torch.nn.functional.linear(o.reshape(o.shape[0], -1), self.o_weight, self.o_bias)
+
+    def prompt(self, x: torch.Tensor, cache, layer: int, rope: tuple[torch.Tensor, torch.Tensor], cu_seqlens: torch.Tensor,
+               positions: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
+        """Whole prompts (packed tokens x [T, H], reserved in ``cache``): writes their keys and values, returns [T, H]."""
+        q, k, v = self.project(x)
+        q, k = rope_append(q, k, v, *rope, positions, rows, cache.k(layer), cache.v(layer), cache.block_table, return_k=True)
+        return self.output(attn_prompt(q, k, v, cu_seqlens, window=self.window, sinks=self.sinks, scale=self.scale))
+
+    def decode(self, x: torch.Tensor, cache, layer: int, rope: tuple[torch.Tensor, torch.Tensor], positions: torch.Tensor,
+               rows: torch.Tensor, group_starts: torch.Tensor | None = None, prefix_lens: torch.Tensor | None = None) -> torch.Tensor:
+        """One token per sequence (x [rows, H], reserved in ``cache``): writes its key and value, returns [rows, H]."""
+        q, k, v = self.project(x)
+        q = rope_append(q, k, v, *rope, positions, rows, cache.k(layer), cache.v(layer), cache.block_table)
+        o = attn_decode(q, cache.k(layer), cache.v(layer), cache.block_table, cache.lens, window=self.window, sinks=self.sinks,
+                        scale=self.scale, group_starts=group_starts, prefix_lens=prefix_lens)
+        return self.output(o)

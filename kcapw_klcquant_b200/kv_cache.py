@@ -100,6 +100,17 @@ class PagedKvCache:
         self._call(_lib.lib().klc_kv_compact, self.live.data_ptr(), self._ws.data_ptr(), self._ws.numel())
         return self.live
 
+    def snapshot(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """The page tables, lengths and reference counts (copies; not the pages' contents): with :meth:`restore`,
+        sequences go back to an earlier length (KVCacheManager.snapshot, kv_cache_manager.py:80-91)."""
+        return self.block_table.clone(), self.lens.clone(), self.refs.clone()
+
+    def restore(self, state: tuple[torch.Tensor, torch.Tensor, torch.Tensor]) -> None:
+        """Back to a :meth:`snapshot`.  Keys up to the restored lengths must still be in their pages: nothing was freed and
+        handed out again, or compacted, since."""
+        for mine, theirs in zip((self.block_table, self.lens, self.refs), state):
+            mine.copy_(theirs)
+
     def check(self) -> None:
         """Raise if a call could not serve a request (synchronises)."""
         check_device_status(self.device)

@@ -20,6 +20,17 @@ computed).  Layers are :class:`MoeLayer` (one GPU) or
 the GPUs of a node); both are free of host synchronisation, so
 :meth:`MoeStack.capture` records a whole decode step of all layers as one CUDA
 graph and :meth:`MoeStack.replay` runs it.
+
+With ``attention`` the stack runs whole layers as the executor does
+(streamed_transformer_executor.py:231-275), over a :class:`PagedKvCache`:
+
+    for every layer L:
+        hidden = hidden + attention_L(rms_norm(hidden, input_norm[L]))
+        hidden = hidden + moe_L(rms_norm(hidden, norm[L]))
+
+:meth:`MoeStack.prompt` takes whole packed prompts, :meth:`MoeStack.step` one
+token for every row of the cache.  Pages are taken and lengths advanced on the
+device, so a captured step can be replayed token after token.
 """
 from __future__ import annotations
 
@@ -32,15 +43,33 @@ class MoeStack:
     """MoE layers with RMSNorm weights ``norm_weights[L]`` (bf16 [H]) applied to each layer's input."""
 
     def __init__(self, layers: list, norm_weights: list[torch.Tensor], eps: float = 1e-5, precision: str = "bf16",
-                 fuse_router: bool = False):
+                 fuse_router: bool = False, attention: list | None = None, input_norm_weights: list[torch.Tensor] | None = None,
+                 cache=None, rope: tuple[torch.Tensor, torch.Tensor] | None = None):
         if len(norm_weights) != len(layers):
             raise ValueError("one RMSNorm weight per layer")
+        if attention is not None:
+            if input_norm_weights is None or cache is None or rope is None:
+                raise ValueError("attention needs input_norm_weights, a cache and the rotary tables")
+            if len(attention) != len(layers) or len(input_norm_weights) != len(layers):
+                raise ValueError("one attention layer and one input norm per layer")
+            if cache.pool.shape[0] < len(layers):
+                raise ValueError("the cache has fewer layers than the stack")
+            if fuse_router:
+                raise ValueError("fuse_router routes the next layer's input before its attention: not with attention")
         self.layers = list(layers)
         dev = self._device()
         self.norm_weights = [as_bf16(w, dev) for w in norm_weights]
         self.eps = float(eps)
         self.precision = precision
         self.fuse_router = bool(fuse_router)
+        self.attention = None if attention is None else list(attention)
+        self.cache = cache
+        if attention is not None:
+            self.input_norm_weights = [as_bf16(w, dev) for w in input_norm_weights]
+            self.rope = tuple(t.to(device=dev, dtype=torch.float32).contiguous() for t in rope)
+            # one token per step and row; rows that sit out: set_active
+            self._add = torch.ones(cache.rows, dtype=torch.int32, device=dev)
+            self._rows = torch.arange(cache.rows, dtype=torch.int32, device=dev)
         self._graph = None
         self._static_in = None
         self._static_out = None
@@ -50,7 +79,10 @@ class MoeStack:
         return first.device if isinstance(first, MoeLayer) else first.backend.device
 
     def step(self, hidden: torch.Tensor) -> torch.Tensor:
-        """One pass of this rank's tokens bf16 [T, H] through every layer."""
+        """One pass of this rank's tokens bf16 [T, H] through every layer (with attention: one token for every row of
+        the cache, T = its rows)."""
+        if self.attention is not None:
+            return self._decode_step(hidden)
         normed = rms_norm(hidden, self.norm_weights[0], self.eps)
         n = len(self.layers)
         idx = w = None  # routing of this layer, when the previous layer's combine computed it
@@ -81,15 +113,77 @@ class MoeStack:
             hidden = y
         return hidden
 
+    def set_active(self, active: torch.Tensor) -> None:
+        """Which rows of the cache take part in :meth:`step` (bool [rows]); the others' keys and lengths stay as they are
+        and their outputs mean nothing.  May be changed between replays of a captured step."""
+        on = active.to(device=self._add.device, dtype=torch.bool)
+        if on.shape != self._add.shape:
+            raise ValueError(f"active must have {self._add.numel()} elements")
+        self._add.copy_(on)
+        self._rows.copy_(torch.where(on, torch.arange(on.numel(), dtype=torch.int32, device=on.device), -1))
+
+    def _layers(self, hidden: torch.Tensor, attend) -> torch.Tensor:
+        """Whole layers; ``attend(layer, normed)`` is the attention of one."""
+        normed = rms_norm(hidden, self.input_norm_weights[0], self.eps)
+        n = len(self.layers)
+        for li, layer in enumerate(self.layers):
+            hidden = hidden + attend(li, normed)
+            post = rms_norm(hidden, self.norm_weights[li], self.eps)
+            nxt = None if li + 1 == n else (self.input_norm_weights[li + 1], self.eps)
+            if nxt is None:
+                hidden, _ = layer.forward(post, precision=self.precision, residual=hidden)
+            elif isinstance(layer, MoeLayer):
+                hidden, rb = layer.forward(post, precision=self.precision, residual=hidden, next_norm=nxt)
+                normed = rb.normed
+            else:
+                hidden, _, normed = layer.forward(post, precision=self.precision, residual=hidden, next_norm=nxt)
+        return hidden
+
+    def _decode_step(self, hidden: torch.Tensor) -> torch.Tensor:
+        cache = self.cache
+        if hidden.shape[0] != cache.rows:
+            raise ValueError(f"a step takes one token for each of the cache's {cache.rows} rows")
+        positions = cache.lens.clone()
+        cache.reserve(self._add)
+        return self._layers(hidden, lambda li, x: self.attention[li].decode(x, cache, li, self.rope, positions, self._rows))
+
+    def prompt(self, hidden: torch.Tensor, cu_seqlens: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
+        """Whole prompts through every layer: packed tokens bf16 [T, H], sequence b the rows ``cu_seqlens[b]:cu_seqlens[b + 1]``
+        (int32 on the device), into the empty cache rows ``rows`` int32 [B].  Returns [T, H]; ``cache.check()`` tells whether
+        the pages sufficed."""
+        if self.attention is None:
+            raise RuntimeError("the stack has no attention layers")
+        T, dev = int(hidden.shape[0]), hidden.device
+        if rows.dim() != 1 or cu_seqlens.shape != (rows.shape[0] + 1,):
+            raise ValueError("cu_seqlens must have one element more than rows")
+        lens = cu_seqlens[1:] - cu_seqlens[:-1]
+        add = torch.zeros_like(self._add)
+        add[rows.long()] = lens
+        self.cache.reserve(add)
+        # tokens past the last sequence are padding: row -1
+        seq = torch.bucketize(torch.arange(T, dtype=torch.int32, device=dev), cu_seqlens[1:], right=True, out_int32=True)
+        inside = seq < rows.shape[0]
+        at = seq.clamp(max=max(rows.shape[0] - 1, 0)).long()
+        positions = torch.arange(T, dtype=torch.int32, device=dev) - cu_seqlens[at]
+        token_rows = torch.where(inside, rows[at], -1).to(torch.int32)
+        return self._layers(hidden, lambda li, x: self.attention[li].prompt(x, self.cache, li, self.rope, cu_seqlens, positions,
+                                                                            token_rows))
+
     def capture(self, example: torch.Tensor, warmup: int = 2) -> None:
-        """Record :meth:`step` on a static input buffer shaped like ``example`` as a CUDA graph."""
+        """Record :meth:`step` on a static input buffer shaped like ``example`` as a CUDA graph.
+
+        With attention the warm-up steps need pages for ``warmup`` tokens in every active row; tables and lengths are put
+        back behind them."""
         self._static_in = example.clone()
+        state = None if self.attention is None else self.cache.snapshot()  # warm-up steps leave the sequences as they were
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             for _ in range(warmup):  # workspaces sized and kernels loaded outside the capture
                 self.step(self._static_in)
         torch.cuda.current_stream().wait_stream(side)
+        if state is not None:
+            self.cache.restore(state)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             self._static_out = self.step(self._static_in)
