@@ -18,12 +18,16 @@ fp32.  All math runs in the CUDA kernels of libklcmoe.so.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 
 import torch
 
 from . import _lib
 from .moe import as_bf16, workspace
+
+# the current stream of a device as an integer, without making a Stream object for it where torch offers that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _lib.stream_ptr)
 
 _STATUS: dict[int, torch.Tensor] = {}
 _STATUS_LOCK = threading.Lock()
@@ -133,7 +137,7 @@ def _device_of(q: torch.Tensor) -> int:
 
 
 class on_device:
-    """``torch.cuda.device`` that costs nothing when the device is current already; gives the current stream."""
+    """``torch.cuda.device`` that costs nothing when the device is current already; gives the device's current stream."""
 
     __slots__ = ("index", "guard")
 
@@ -145,11 +149,20 @@ class on_device:
         if torch.cuda.current_device() != self.index:
             self.guard = torch.cuda.device(self.index)
             self.guard.__enter__()
-        return _lib.stream_ptr(self.index)
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc) -> None:
         if self.guard is not None:
             self.guard.__exit__(*exc)
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_bytes(dtype: int, heads: int, kv_heads: int, d: int, batch: int, groups: int, device: int) -> int:
+    """Workspace of a decode call of these sizes (asked of the library once per set of sizes)."""
+    n = ctypes.c_size_t(0)
+    dims = _lib.KlcAttnDims(dtype, heads, kv_heads, d, 0, 1.0)
+    _lib.check(_lib.lib().klc_attn_decode_workspace_size(ctypes.byref(dims), batch, groups, ctypes.byref(n)))
+    return n.value
 
 
 def attn_prompt(
@@ -297,9 +310,7 @@ def attn_decode(
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     L = _lib.lib()
     with on_device(dev) as stream:
-        n = ctypes.c_size_t(0)
-        _lib.check(L.klc_attn_decode_workspace_size(ctypes.byref(dims), B, groups, ctypes.byref(n)))
-        ws = _workspace(q.device, n.value, stream)
+        ws = _workspace(q.device, _decode_bytes(dims.dtype, dims.heads, kv_heads, d, B, groups, dev), stream)
         _lib.check(L.klc_attn_decode(
             ctypes.byref(dims), *qa, k_pages.data_ptr(), v_pages.data_ptr(), pages, ps, page_stride, block_table.data_ptr(), width,
             table_stride, ln.data_ptr(), B, _lib.ptr(gs), _lib.ptr(pl), groups, _lib.ptr(sk), *oa, _lib.ptr(lse), ws.data_ptr(),

@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cmath>
 
 #include "klc_common.cuh"
@@ -82,6 +83,20 @@ inline int check_scale(const char* who, float scale) {
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail(KLC_ERR_INVALID, std::string(who) + ": scale must be finite and > 0");
   return KLC_OK;
 }
+
+// Raises a kernel's dynamic shared memory limit, once per device (a call on each launch costs host time).
+struct SmemLimit {
+  std::atomic<uint64_t> done{0};  // bit d: device d
+  int raise(const void* kernel, size_t bytes) {
+    int dev = 0;
+    KLC_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (bit != 0 && (done.load(std::memory_order_relaxed) & bit) != 0) return KLC_OK;
+    KLC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return KLC_OK;
+  }
+};
 
 inline bool page_size_ok(int ps) { return ps == 16 || ps == 32 || ps == 64 || ps == 128; }
 

@@ -553,7 +553,9 @@ template <typename T, int D>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const DecodeParams& p, int ctas, cudaStream_t s) {
   const size_t smem = DCfg<D>::smem(p.batch);
   auto kernel = attn_decode_kernel<T, D>;
-  KLC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  static SmemLimit limit;
+  int st = limit.raise(reinterpret_cast<const void*>(kernel), DCfg<D>::smem(kMaxBatch));
+  if (st != KLC_OK) return st;
   KLC_CUDA(launch_chain(kernel, dim3(unsigned(ctas)), dim3(kThreads), smem, s, 0, mk, mv, p));
   KLC_LAUNCH_CHECK("attn_decode");
   const int64_t rows = int64_t(p.batch) * p.heads;

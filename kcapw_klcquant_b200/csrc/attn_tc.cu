@@ -722,7 +722,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             tmem_wait_ld32(s0);
             float s1[32];
             tmem_ld32(s_col + 32, s1);
-            if (i > 0) ok = wait_bar_short(o_full(t), (steps - 1) & 1, ctl, 517);  // the previous P V still reads P till then
+            if (i > 0) {  // the previous P V still reads P till then
+              ok = wait_bar_short(o_full(t), (steps - 1) & 1, ctl, 517);
+              ok = __all_sync(0xffffffffu, ok);
+              tc_fence_after();
+            }
             tmem_st32(p_col + 32, pk);
             hide(s0, 0);
             numerators(s0, pk, whole);
@@ -760,7 +764,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(p_full(t));
-        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        if (!ok) break;
       }
       // ---- epilogue: the row's output
       if (ok && it.n > 0) {
@@ -831,7 +835,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 template <typename T, int D, bool PREFIX>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& p, int64_t items, cudaStream_t s) {
   auto kernel = attn_tc_kernel<T, D, PREFIX>;
-  KLC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
+  static SmemLimit limit;
+  int st = limit.raise(reinterpret_cast<const void*>(kernel), Cfg<D>::kSmem);
+  if (st != KLC_OK) return st;
   kernel<<<unsigned(std::min<int64_t>(items, sm_count())), kThreads, Cfg<D>::kSmem, s>>>(mq, mk, mv, p);
   KLC_LAUNCH_CHECK(PREFIX ? "attn_prefix" : "attn_prompt");
   return KLC_OK;

@@ -8,6 +8,8 @@
 // more than fp32 before the cosine is taken, so the caller makes them in
 // fp64, once).  Bytes bound it: q, k, v are read once, q and the pages written
 // once.  A thread rotates eight pairs (two 16-byte loads and stores) or copies eight values.
+#include <algorithm>
+
 #include "attn_common.cuh"
 #include "attn_kernels.cuh"
 
@@ -16,6 +18,7 @@ namespace attn {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMaxTokens = 8;  // tokens a block
 
 struct RopeParams {
   const void *q, *k, *v;
@@ -50,76 +53,86 @@ __device__ __forceinline__ void rotate8(const uint4& a, const uint4& b, const fl
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeParams p, int block_tokens) {
   constexpr int kPairs = D / 16, kVals = D / 8;  // threads a head's rotation / copy takes
+  __shared__ int64_t slot_s[kMaxTokens];         // of the token's first key head in the pools; -1: no place, -2: write nothing
+  __shared__ int pos_s[kMaxTokens];
   pdl_trigger();
   pdl_wait();
-  const int rot = (p.heads + p.kv_heads) * kPairs, per_token = rot + p.kv_heads * kVals;
-  const int64_t idx = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t t = idx / per_token;
-  if (t >= p.tokens) return;
-  const int u = int(idx - t * per_token);
-  const int row = p.rows[t];
-  if (row == -1) return;  // padding: nothing of it is written
-  const int pos = p.pos[t];
-  if (row < 0 || row >= p.table_rows || pos < 0 || pos >= p.max_pos || pos / p.page_size >= p.table_width) {
-    record_fault(p.status, KLC_ERR_DEVICE_FAULT, 540, int(t));
-    return;
-  }
-  const bool is_q = u < p.heads * kPairs;
-  int64_t slot = 0;  // of the token's first key head in the pools
-  if (!is_q) {
-    const int page = p.table[int64_t(row) * p.table_stride + pos / p.page_size];
-    if (page < 0 || page >= p.pages) {
-      record_fault(p.status, KLC_ERR_DEVICE_FAULT, 541, page);
-      return;
-    }
-    slot = int64_t(page) * p.page_stride + int64_t(pos % p.page_size) * D;
-  }
-  const int64_t head_pitch = int64_t(p.page_size) * D;
-  if (u < rot) {
-    const int head = u / kPairs, part = u - head * kPairs;  // eight pairs from column 8 * part
-    const int kh = head - p.heads;
-    const T* src = (is_q ? reinterpret_cast<const T*>(p.q) + t * p.q_ts + int64_t(head) * p.q_hs
-                         : reinterpret_cast<const T*>(p.k) + t * p.k_ts + int64_t(kh) * p.k_hs) +
-                   part * 8;
-    const uint4 a = *reinterpret_cast<const uint4*>(src), b = *reinterpret_cast<const uint4*>(src + D / 2);
-    float c[8], s[8];
-    const int64_t ang = int64_t(pos) * (D / 2) + part * 8;
-#pragma unroll
-    for (int j = 0; j < 8; j += 4) {
-      *reinterpret_cast<float4*>(c + j) = *reinterpret_cast<const float4*>(p.cos + ang + j);
-      *reinterpret_cast<float4*>(s + j) = *reinterpret_cast<const float4*>(p.sin + ang + j);
-    }
-    uint4 oa, ob;
-    rotate8<T>(a, b, c, s, &oa, &ob);
-    if (is_q) {
-      T* dst = reinterpret_cast<T*>(p.q_out) + t * p.qo_ts + int64_t(head) * p.qo_hs + part * 8;
-      *reinterpret_cast<uint4*>(dst) = oa;
-      *reinterpret_cast<uint4*>(dst + D / 2) = ob;
-    } else {
-      T* dst = reinterpret_cast<T*>(p.k_pages) + slot + kh * head_pitch + part * 8;
-      *reinterpret_cast<uint4*>(dst) = oa;
-      *reinterpret_cast<uint4*>(dst + D / 2) = ob;
-      if (p.k_out != nullptr) {
-        T* ko = reinterpret_cast<T*>(p.k_out) + t * p.ko_ts + int64_t(kh) * p.ko_hs + part * 8;
-        *reinterpret_cast<uint4*>(ko) = oa;
-        *reinterpret_cast<uint4*>(ko + D / 2) = ob;
+  const int64_t t0 = int64_t(blockIdx.x) * block_tokens;
+  const int n = int(min(int64_t(block_tokens), p.tokens - t0));
+  if (threadIdx.x < n) {
+    const int64_t t = t0 + threadIdx.x;
+    const int row = p.rows[t], pos = p.pos[t];
+    int64_t slot = -2;  // row -1 is padding
+    if (row != -1) {
+      if (row < 0 || row >= p.table_rows || pos < 0 || pos >= p.max_pos || pos / p.page_size >= p.table_width) {
+        record_fault(p.status, KLC_ERR_DEVICE_FAULT, 540, int(t));
+      } else {
+        const int page = p.table[int64_t(row) * p.table_stride + pos / p.page_size];
+        slot = -1;
+        if (page < 0 || page >= p.pages) record_fault(p.status, KLC_ERR_DEVICE_FAULT, 541, page);
+        else slot = int64_t(page) * p.page_stride + int64_t(pos % p.page_size) * D;
       }
     }
-  } else {
-    const int w = u - rot, kh = w / kVals, part = w - kh * kVals;
-    const T* src = reinterpret_cast<const T*>(p.v) + t * p.v_ts + int64_t(kh) * p.v_hs + part * 8;
-    *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.v_pages) + slot + kh * head_pitch + part * 8) =
-        *reinterpret_cast<const uint4*>(src);
+    slot_s[threadIdx.x] = slot;
+    pos_s[threadIdx.x] = pos;
+  }
+  __syncthreads();
+  const int rot = (p.heads + p.kv_heads) * kPairs, per_token = rot + p.kv_heads * kVals;
+  const int64_t head_pitch = int64_t(p.page_size) * D;
+#pragma unroll 2
+  for (int i = threadIdx.x; i < n * per_token; i += kThreads) {
+    const int j = i / per_token, u = i - j * per_token;
+    const int64_t slot = slot_s[j], t = t0 + j;
+    const bool is_q = u < p.heads * kPairs;
+    if (slot == -2 || (slot == -1 && !is_q)) continue;
+    if (u < rot) {
+      const int head = u / kPairs, part = u - head * kPairs;  // eight pairs from column 8 * part
+      const int kh = head - p.heads;
+      const T* src = (is_q ? reinterpret_cast<const T*>(p.q) + t * p.q_ts + int64_t(head) * p.q_hs
+                           : reinterpret_cast<const T*>(p.k) + t * p.k_ts + int64_t(kh) * p.k_hs) +
+                     part * 8;
+      const uint4 a = *reinterpret_cast<const uint4*>(src), b = *reinterpret_cast<const uint4*>(src + D / 2);
+      float c[8], s[8];
+      const int64_t ang = int64_t(pos_s[j]) * (D / 2) + part * 8;
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        *reinterpret_cast<float4*>(c + e) = *reinterpret_cast<const float4*>(p.cos + ang + e);
+        *reinterpret_cast<float4*>(s + e) = *reinterpret_cast<const float4*>(p.sin + ang + e);
+      }
+      uint4 oa, ob;
+      rotate8<T>(a, b, c, s, &oa, &ob);
+      if (is_q) {
+        T* dst = reinterpret_cast<T*>(p.q_out) + t * p.qo_ts + int64_t(head) * p.qo_hs + part * 8;
+        *reinterpret_cast<uint4*>(dst) = oa;
+        *reinterpret_cast<uint4*>(dst + D / 2) = ob;
+      } else {
+        T* dst = reinterpret_cast<T*>(p.k_pages) + slot + kh * head_pitch + part * 8;
+        *reinterpret_cast<uint4*>(dst) = oa;
+        *reinterpret_cast<uint4*>(dst + D / 2) = ob;
+        if (p.k_out != nullptr) {
+          T* ko = reinterpret_cast<T*>(p.k_out) + t * p.ko_ts + int64_t(kh) * p.ko_hs + part * 8;
+          *reinterpret_cast<uint4*>(ko) = oa;
+          *reinterpret_cast<uint4*>(ko + D / 2) = ob;
+        }
+      }
+    } else {
+      const int w = u - rot, kh = w / kVals, part = w - kh * kVals;
+      const T* src = reinterpret_cast<const T*>(p.v) + t * p.v_ts + int64_t(kh) * p.v_hs + part * 8;
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.v_pages) + slot + kh * head_pitch + part * 8) =
+          *reinterpret_cast<const uint4*>(src);
+    }
   }
 }
 
 template <typename T, int D>
 int launch(const RopeParams& p, cudaStream_t s) {
-  const int64_t units = p.tokens * (int64_t(p.heads + p.kv_heads) * (D / 16) + int64_t(p.kv_heads) * (D / 8));
-  KLC_CHECK_ARG(units / kThreads < (int64_t(1) << 31) - 1, "klc_rope_append: too many tokens for one call");
-  KLC_CUDA(launch_chain(rope_append_kernel<T, D>, dim3(unsigned((units + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, 0, p));
+  // enough blocks to fill the SMs eight times over, up to kMaxTokens tokens each
+  const int64_t bt = std::max<int64_t>(1, std::min<int64_t>(kMaxTokens, p.tokens / (int64_t(sm_count()) * 8)));
+  const int64_t blocks = (p.tokens + bt - 1) / bt;
+  KLC_CHECK_ARG(blocks < (int64_t(1) << 31), "klc_rope_append: too many tokens for one call");
+  KLC_CUDA(launch_chain(rope_append_kernel<T, D>, dim3(unsigned(blocks)), dim3(kThreads), 0, s, 0, p, int(bt)));
   KLC_LAUNCH_CHECK("rope_append");
   return KLC_OK;
 }
