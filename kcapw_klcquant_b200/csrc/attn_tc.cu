@@ -637,6 +637,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       }
       // the row reaches these tiles whole: rows that are not there do not make a tile a boundary one
       const int wlo = __reduce_max_sync(0xffffffffu, row_ok ? jlo : 0), whi = __reduce_min_sync(0xffffffffu, row_ok ? jhi : 0x7fffffff);
+      const int head = it.kvh * G + g;
+      const float sink = !PREFIX && row_ok && p.sinks != nullptr ? p.sinks[head] * kLog2e : 0.f;  // used at the end
       float m = -INFINITY, l = 0.f;  // m: reference maximum (log2 units) of the stored P and O
       bool ok = true;
       for (int i = 0; i < it.n; ++i, ++steps) {
@@ -652,19 +654,44 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         tmem_ld64(s_col, sa);
         tmem_wait_ld64(sa);
         tmem_ld64(s_col + 64, sb);
-        if (masked) {
+        // boundary tiles, 32 columns at a time: bit c, no row of the warp sees any / some row does not see all of columns 32 c ..
+        // (D = 64: 2 to 6 % on ragged and windowed prompts; with D = 128 it cost 2 % in registers)
+        uint32_t none = 0, part = masked ? 15u : 0u;
+        if (C::kOwnP && masked) {
+          part = 0;
 #pragma unroll
-          for (int j = 0; j < 64; ++j) sa[j] = (j >= ja && j <= jb) ? sa[j] : -INFINITY;
+          for (int c = 0; c < 4; ++c) {
+            if (!__any_sync(0xffffffffu, ja <= 32 * c + 31 && jb >= 32 * c)) none |= 1u << c;
+            if (__any_sync(0xffffffffu, row_ok && (ja > 32 * c || jb < 32 * c + 31))) part |= 1u << c;
+          }
+          part &= ~none;
         }
+        auto hide = [&](float* s, int c) {
+          if (part >> c & 1) {
 #pragma unroll
-        for (int j = 0; j < 64; j += 2) mx[(j >> 1) & 3] = max3_nan(mx[(j >> 1) & 3], sa[j], sa[j + 1]);
+            for (int j = 0; j < 32; ++j) s[j] = (32 * c + j >= ja && 32 * c + j <= jb) ? s[j] : -INFINITY;
+          } else if (none >> c & 1) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s[j] = -INFINITY;
+          }
+        };
+        auto peak = [&](const float* s) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) mx[(j >> 1) & 3] = max3_nan(mx[(j >> 1) & 3], s[j], s[j + 1]);
+        };
+        if (masked) {
+          hide(sa, 0);
+          hide(sa + 32, 1);
+        }
+        peak(sa);
+        peak(sa + 32);
         tmem_wait_ld64(sb);
         if (masked) {
-#pragma unroll
-          for (int j = 0; j < 64; ++j) sb[j] = (64 + j >= ja && 64 + j <= jb) ? sb[j] : -INFINITY;
+          hide(sb, 2);
+          hide(sb + 32, 3);
         }
-#pragma unroll
-        for (int j = 0; j < 64; j += 2) mx[(j >> 1) & 3] = max3_nan(mx[(j >> 1) & 3], sb[j], sb[j + 1]);
+        peak(sb);
+        peak(sb + 32);
         const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;
         // the reference moves when the maximum has grown by more than 2^8 (or to a NaN)
         const bool grow = row_ok && (m == -INFINITY ? top != -INFINITY : !(top <= m + kRescaleLog2));
@@ -709,11 +736,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           }
         };
         auto write_p = [&](auto whole) {
-          auto hide = [&](float* s, int c) {
-            if (!decltype(whole)::value) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) s[j] = (c + j >= ja && c + j <= jb) ? s[j] : -INFINITY;
-            }
+          auto hide_again = [&](float* s, int c) {
+            if (!decltype(whole)::value) hide(s, c);
           };
           if constexpr (C::kOwnP) {
             uint32_t pk[32];
@@ -728,12 +752,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
               tc_fence_after();
             }
             tmem_st32(p_col + 32, pk);
-            hide(s0, 0);
+            hide_again(s0, 0);
             numerators(s0, pk, whole);
             tmem_wait_ld32(s1);
             tc_fence_before();
             mbar_arrive(s_free(t));
-            hide(s1, 32);
+            hide_again(s1, 1);
             numerators(s1, pk + 16, whole);
             tmem_st32(p_col, pk);
           } else {
@@ -748,11 +772,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             tmem_wait_st();  // keys 64-127: their half of the product starts here
             tc_fence_before();
             mbar_arrive(p_half(t));
-            hide(s0, 0);
+            hide_again(s0, 0);
             numerators(s0, pk, whole);
             tmem_st16(p_col, pk);
             tmem_wait_ld32(s1);
-            hide(s1, 32);
+            hide_again(s1, 1);
             numerators(s1, pk, whole);
             tmem_st16(p_col + 16, pk);
           }
@@ -774,7 +798,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       }
       if (!ok) break;
       const int64_t row = int64_t(it.q0) + tok;
-      const int head = it.kvh * G + g;
       if (PREFIX) {
         const int64_t slot = (int64_t(it.z) * p.total_q + row) * p.heads + head;
         if (row_ok) p.part_ml[slot] = make_float2(m, l);
@@ -792,10 +815,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           }
         }
       } else {
-        const bool has_sink = p.sinks != nullptr;
         float inv = 0.f, lse = 0.f;
         if (row_ok) {
-          finish_row(m, l, has_sink, has_sink ? p.sinks[head] * kLog2e : 0.f, &inv, &lse);
+          finish_row(m, l, p.sinks != nullptr, sink, &inv, &lse);
           if (p.lse != nullptr) p.lse[row * p.heads + head] = lse;
         }
         uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + row * p.out_ts + int64_t(head) * p.out_hs);
