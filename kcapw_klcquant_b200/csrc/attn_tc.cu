@@ -881,6 +881,9 @@ CUtensorMapDataType map_type(int dtype) {
 // rows [tokens][heads][D] with token / head strides in elements; box of `box_heads` x `box_tokens`
 int rows_map(CUtensorMap* m, int dtype, int head_dim, const void* base, int64_t tokens, int heads, int64_t ts, int64_t hs,
              int box_heads, int box_tokens) {
+  // the stride of a dimension of one means nothing, but the map wants one
+  if (heads == 1) hs = head_dim;
+  if (tokens <= 1) ts = hs * heads;
   const uint64_t dims[3] = {uint64_t(head_dim), uint64_t(heads), uint64_t(tokens)};
   const uint64_t strides[2] = {uint64_t(hs) * 2, uint64_t(ts) * 2};
   const uint32_t box[3] = {64, uint32_t(box_heads), uint32_t(box_tokens)};
@@ -983,7 +986,7 @@ extern "C" int klc_attn_prompt(const klc_attn_dims* dims, const void* q, int64_t
   p.group = G;
   p.tpt = kRows / G;
   p.scale_log2 = dims->scale * kLog2e;
-  p.window = dims->window;
+  p.window = std::min(dims->window, 1 << 30);  // no position is larger, and position - window stays in 32 bits
   p.sinks = sinks;
   p.out = out;
   p.out_ts = out_token_stride;

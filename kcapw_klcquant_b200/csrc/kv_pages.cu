@@ -407,6 +407,7 @@ int check_cache(const klc_kv_cache* c, const std::string& w) {
   KLC_CHECK_ARG(page_size_ok(c->page_size), w + ": page_size must be 16, 32, 64 or 128");
   KLC_CHECK_ARG(c->table_width >= 0 && c->table_width < (int64_t(1) << 31) && c->table_stride >= c->table_width && c->table_width * c->page_size < (int64_t(1) << 31),
                 w + ": bad block table width or stride");
+  KLC_CHECK_ARG(c->rows * c->table_width < (int64_t(1) << 31), w + ": the block table is too large");  // pages asked for at once
   KLC_CHECK_ARG(c->planes >= 0 && c->page_bytes > 0 && c->page_bytes % 16 == 0 && c->plane_stride % 16 == 0,
                 w + ": page_bytes and plane_stride must be multiples of 16");
   KLC_CHECK_ARG(c->planes <= 1 || c->plane_stride >= c->pages * c->page_bytes, w + ": plane_stride must hold all pages");

@@ -97,7 +97,8 @@ def kv(**kw):
 
 @pytest.mark.parametrize("bad", [dict(pages=0), dict(rows=-1), dict(page_size=48), dict(table_stride=3), dict(page_bytes=0), dict(page_bytes=4104),
                                  dict(plane_stride=4096), dict(refs=None), dict(refs=A + 4), dict(lens=None), dict(block_table=None), dict(pool=None),
-                                 dict(pool=A + 8), dict(table_width=1 << 31, table_stride=1 << 31)])
+                                 dict(pool=A + 8), dict(table_width=1 << 31, table_stride=1 << 31),
+                                 dict(rows=1 << 20, table_width=1 << 12, table_stride=1 << 12)])
 def test_cache_refusals(bad):
     L, c = _lib.lib(), kv(**bad)
     big = 1 << 20

@@ -63,6 +63,63 @@ def test_prompt_other_keys(dtype, d, lq, lk, window):
     check_prompt(q, k, v, lq, lk, window, None, out, lse, 0.2)
 
 
+@pytest.mark.parametrize("window", [1 << 30, (1 << 31) - 1])
+def test_largest_windows(window):
+    """A window larger than any position is none, also for rows before the first key."""
+    from kcapw_klcquant_b200 import attn_decode, attn_prompt
+
+    q, k, v = rnd((200, 4, 64), BF, 2), rnd((70, 2, 64), BF, 3), rnd((70, 2, 64), BF, 4)
+    a = attn_prompt(q, k, v, cum([200]), cu_seqlens_k=cum([70]))
+    assert torch.equal(attn_prompt(q, k, v, cum([200]), cu_seqlens_k=cum([70]), window=window), a)
+    kp, vp, table = ref.paged([k], [v], 16)
+    ln = torch.tensor([70], dtype=torch.int32, device=DEV)
+    a = attn_decode(q[:1], kp, vp, table, ln)
+    assert torch.equal(attn_decode(q[:1], kp, vp, table, ln, window=window), a)
+
+
+def test_prompt_output_over_the_queries_and_single_heads():
+    from kcapw_klcquant_b200 import attn_prompt
+
+    lens = [130, 61]
+    q, k, v = rnd((191, 1, 128), HF, 2), rnd((191, 1, 128), HF, 3), rnd((191, 1, 128), HF, 4)
+    want = attn_prompt(q, k, v, cum(lens))
+    assert attn_prompt(q, k, v, cum(lens), out=q) is q and torch.equal(q, want)
+
+
+def test_prompt_captured_serves_other_offsets():
+    from kcapw_klcquant_b200 import attn_prompt
+
+    q, k, v = rnd((300, 8, 64), BF, 2), rnd((300, 2, 64), BF, 3), rnd((300, 2, 64), BF, 4)
+    cu = cum([100, 150, 50])
+    attn_prompt(q, k, v, cu)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = attn_prompt(q, k, v, cu)
+    for lens in ([100, 150, 50], [1, 0, 299], [300, 0, 0]):
+        cu.copy_(cum(lens))
+        g.replay()
+        check_prompt(q, k, v, lens, lens, 0, None, out, None, 0.125)
+
+
+def test_calls_on_a_stream_that_is_not_current_at_creation():
+    """Inputs made on one stream, used on another after an event; two prompts in flight at once."""
+    from kcapw_klcquant_b200 import attn_prompt
+
+    q, k, v = rnd((2000, 8, 128), BF, 2), rnd((2000, 2, 128), BF, 3), rnd((2000, 2, 128), BF, 4)
+    want = attn_prompt(q, k, v, cum([1500, 500]))
+    cu = cum([1500, 500])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    outs = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(attn_prompt(q, k, v, cu))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
 def test_prompt_no_keys_at_all_and_no_rows():
     from kcapw_klcquant_b200 import attn_prompt
 
@@ -330,6 +387,42 @@ def test_decode_offsets_past_32_bits():
     q = rnd((1, 16, d), BF, 6)
     out = attn_decode(q, pool, pool, torch.tensor([ids], dtype=torch.int32, device=DEV), torch.tensor([n], dtype=torch.int32, device=DEV))
     check_decode(q, [k], [k], 0, None, out, None)
+
+
+def test_decode_table_slices_and_page_strides():
+    """The layers of one pool (pages far apart), a table that is a slice of a wider one, q a slice of a projection."""
+    from kcapw_klcquant_b200 import attn_decode
+
+    lens = [200, 77]
+    q, ks, vs, _ = decode_case(BF, 6, 2, 64, lens, 32, 0, False)
+    kp, vp, table = ref.paged(ks, vs, 32)
+    pool = torch.full((kp.shape[0], 3, *kp.shape[1:]), float("nan"), dtype=BF, device=DEV)
+    pool[:, 0], pool[:, 2] = kp, vp
+    wide = torch.full((2, table.shape[1] + 9), -5, dtype=torch.int32, device=DEV)
+    wide[:, 2:2 + table.shape[1]] = table
+    qkv = rnd((2, 10, 64), BF, 77)
+    qkv[:, :6] = q
+    out = attn_decode(qkv[:, :6], pool[:, 0], pool[:, 2], wide[:, 2:2 + table.shape[1]], torch.tensor(lens, dtype=torch.int32, device=DEV))
+    check_decode(q, ks, vs, 0, None, out, None)
+
+
+def test_decode_groups_cover_nothing_or_everything():
+    """Zero-length prefixes, empty groups, no groups at all, and bad prefixes reported."""
+    from kcapw_klcquant_b200 import KlcError, attn_decode, check_device_status
+
+    lens = [100, 50, 300]
+    q, ks, vs, _ = decode_case(BF, 8, 2, 64, lens, 16, 0, False)
+    kp, vp, table = ref.paged(ks, vs, 16)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    ln = i32(lens)
+    for gs, pl in (([0, 3], [0]), ([0, 0, 1, 1], [16, 32, 16]), ([0], []), ([2, 3], [160])):
+        out = attn_decode(q, kp, vp, table, ln, group_starts=i32(gs), prefix_lens=i32(pl))
+        check_device_status(DEV)
+        check_decode(q, ks, vs, 0, None, out, None)
+    for gs, pl in (([0, 1], [15]), ([0, 1], [-16]), ([0, 1], [16 * 1000]), ([0, 9], [16]), ([2, 1], [16])):
+        attn_decode(q, kp, vp, table, ln, group_starts=i32(gs), prefix_lens=i32(pl))
+        with pytest.raises(KlcError):
+            check_device_status(DEV)
 
 
 def test_decode_long_context():
