@@ -466,11 +466,13 @@ int klc_status_bytes(size_t* out_bytes);
  * ascending; cu_q may be passed for both).  The last query row sees the last
  * key: with more keys than queries the first keys are an earlier part of the
  * sequence.  Token and head strides are in elements, multiples of 8; rows are
- * 16-byte aligned.  lse fp32 [q_tokens, heads] or NULL.  Rows of q past
- * cu_q[batch] are not written.  A non-finite value row of a sequence's own
- * keys may reach up to 127 rows before it.  Offsets that leave the tensors are
- * recorded as KLC_ERR_DEVICE_FAULT and the sequence is skipped.  Replaces
- * StreamedAttention.forward's loop over the tokens of a prompt.             */
+ * 16-byte aligned.  lse fp32 [q_tokens, heads] or NULL.  Rows of out past
+ * cu_q[batch] are not written; out may be q.  A value (of v) of the sequence's
+ * own that is not finite reaches every row whose key tiles (128 keys) contain
+ * it, seen or not; other sequences' rows and padding reach nothing.  Offsets
+ * that leave the tensors are recorded as KLC_ERR_DEVICE_FAULT and the sequence
+ * is skipped.  Replaces StreamedAttention.forward's loop over the tokens of a
+ * prompt.                                                                   */
 int klc_attn_prompt(const klc_attn_dims* dims, const void* q, int64_t q_tokens, int64_t q_token_stride,
                     int64_t q_head_stride, const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
                     int64_t v_token_stride, int64_t v_head_stride, int64_t k_tokens, const int32_t* cu_q,
@@ -487,7 +489,9 @@ int klc_attn_prompt(const klc_attn_dims* dims, const void* q, int64_t q_tokens, 
  * Shared prefixes: `groups` > 0 groups of consecutive rows, group g the rows
  * group_starts[g] .. group_starts[g+1] (int32 on the device, ascending), whose
  * first prefix_lens[g] keys (a multiple of page_size) are the same pages: they
- * are read once for the whole group, through the table of its first row; rows outside the groups have none.
+ * are read once for the whole group, through the table of its first row; rows
+ * outside the groups have none.  (A prefix value that is not finite may reach
+ * every row of its group, a window or not.)
  * The split over SMs is made on the device from lens, so a captured call
  * serves other lengths on replay.  Results do not depend on timing.  A page id
  * outside [0, pages) and a length outside [0, table_width * page_size] are

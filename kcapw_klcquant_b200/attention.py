@@ -186,7 +186,7 @@ def attn_prompt(
     first keys are an earlier part of the sequence.  ``window`` w > 0 limits a
     row to its last w keys; ``sinks`` fp32 [heads] adds one logit per head to
     the denominator.  q, k and v may be slices of one projection.  Rows of
-    ``out`` past the last sequence are not written.  Returns out [T, heads, D]
+    ``out`` (which may be q) past the last sequence are not written.  Returns out [T, heads, D]
     (and the log-sum-exp fp32 [T, heads] with ``return_lse``).
     """
     dev = _device_of(q)

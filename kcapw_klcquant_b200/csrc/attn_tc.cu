@@ -14,12 +14,18 @@
 //   8, 10     MMA issuer of row tile 0 / 1 (one thread); zeroes value rows past the keys' end
 //   9         finds the items; TMA producer (queries, then a ring of key and value tiles)
 // Per key tile and row tile: S = Q K^T into TMEM (128 fp32 columns), the
-// softmax thread reads its row, writes P as 16-bit pairs over S, and O += P V
+// softmax thread reads its row and writes P as 16-bit pairs, and O += P V
 // reads P from TMEM.  The tensor pipe works on one row tile while the other is
 // in its softmax.  Row statistics are fp32.  O is rescaled only when a row's
 // maximum has grown by more than 2^8 since the last rescale: until then P is at most
-// 2^8, far inside both types' range, and its relative rounding (2^-9 / 2^-12,
+// 2^8, far inside both types' range, and its relative rounding (2^-8 / 2^-11,
 // the price of a 16-bit P operand) does not depend on the reference maximum.
+//
+// Bound: with D = 128 the chain softmax -> P V -> next S of a row tile (TMEM
+// has no room for a second S), with D = 64 the softmax's instructions.  16221
+// tokens, 32 / 8 heads of 128: 2.04 ms, 1.06 PFLOP/s, 62 % of the burst rate of
+// a library product (73 % of its sustained one); 6016 tokens, 64 / 8 heads of
+// 64: 410 us, 725 TFLOP/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -162,8 +168,8 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 
 // 2^x on the FMA pipe, for the share of a tile's exponentials that the special-function unit (16 a clock
 // and SM) would be late with: x = n + f, n the nearest integer (rounded by adding 1.5 * 2^23), 2^f a
-// polynomial fitted on [-1/2, 1/2] (relative error 7.5e-5, degree 3, beside bf16's 2^-9; 2.6e-6,
-// degree 4, beside f16's 2^-12), n added to the exponent.  x below -126 counts as -126.
+// polynomial fitted on [-1/2, 1/2] (relative error 7.5e-5, degree 3, beside bf16's 2^-8; 2.6e-6,
+// degree 4, beside f16's 2^-11), n added to the exponent.  x below -126 counts as -126.
 template <typename T>
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
   const float2 big = make_float2(12582912.f, 12582912.f);

@@ -9,7 +9,8 @@
 //
 // One block makes the plan (it needs global order: prefix sums over the requests
 // and over the free pages; 16 reference counts a thread and step, and the scan stops at the last page
-// that is needed), then a grid moves page contents.  Contents are what costs: 2 x the moved bytes.
+// that is needed), then a grid moves page contents.  Contents are what costs:
+// 2 x the moved bytes (204 pages of 1 MB: 70 us, 6.1 TB/s; a reservation for 48 rows takes 4 us, a fork's plan 10 us).
 #include <algorithm>
 
 #include "attn_common.cuh"
