@@ -467,12 +467,13 @@ int klc_status_bytes(size_t* out_bytes);
  * key: with more keys than queries the first keys are an earlier part of the
  * sequence.  Token and head strides are in elements, multiples of 8; rows are
  * 16-byte aligned.  lse fp32 [q_tokens, heads] or NULL.  Rows of out past
- * cu_q[batch] are not written; out may be q.  A value (of v) of the sequence's
- * own that is not finite reaches every row whose key tiles (128 keys) contain
- * it, seen or not; other sequences' rows and padding reach nothing.  Offsets
- * that leave the tensors are recorded as KLC_ERR_DEVICE_FAULT and the sequence
- * is skipped.  Replaces StreamedAttention.forward's loop over the tokens of a
- * prompt.                                                                   */
+ * cu_q[batch] are not written; out may be q.  Keys and values that no row
+ * sees (padding, other sequences' rows, keys before every window) may hold
+ * anything.  A value of the sequence's own that is not finite reaches the rows
+ * that see it and may reach the others of their 256 / G neighbouring tokens (G
+ * query heads per key head).  Offsets that leave the tensors are recorded as
+ * KLC_ERR_DEVICE_FAULT and the sequence is skipped.  Replaces StreamedAttention.forward's loop over the tokens of a
+ * prompt. */
 int klc_attn_prompt(const klc_attn_dims* dims, const void* q, int64_t q_tokens, int64_t q_token_stride,
                     int64_t q_head_stride, const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
                     int64_t v_token_stride, int64_t v_head_stride, int64_t k_tokens, const int32_t* cu_q,

@@ -11,7 +11,7 @@
 // sequences fill tiles that 128 tokens of one head would not.  Keys come in
 // tiles of 128.  Warps:
 //   0-3, 4-7  softmax of row tile 0 / 1, one row per thread (TMEM lane = row)
-//   8, 10     MMA issuer of row tile 0 / 1 (one thread); zeroes value rows past the keys' end
+//   8, 10     MMA issuer of row tile 0 / 1 (one thread); zeroes value rows that no row of the item sees
 //   9         finds the items; TMA producer (queries, then a ring of key and value tiles)
 // Per key tile and row tile: S = Q K^T into TMEM (128 fp32 columns), the
 // softmax thread reads its row and writes P as 16-bit pairs, and O += P V
@@ -243,6 +243,7 @@ struct Item {
   int tiles;   // row tiles with rows: 1 or 2
   int lo, n;   // key tiles lo .. lo + n
   int kvh, z;  // key head; prefix: share of the keys
+  int first, last;  // lowest and highest key that some row of the item sees
 };
 
 template <int D>
@@ -364,7 +365,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       const int64_t idx = int64_t(wave) * gridDim.x + ((wave & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
       const int64_t pair = idx / unit;
       const int sub = int(idx - pair * unit);
-      Item it{0, 0, 0, 0, -1, 0, 0, 0, 0, 0};
+      Item it{0, 0, 0, 0, -1, 0, 0, 0, 0, 0, 0, 0};
       for (; seq0 < p.batch; seq0 += 32) {
         const int s = seq0 + lane;
         int qb = 0, qn = 0, kb = 0, kn = 0;
@@ -438,6 +439,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
         it.lo = lo;
         it.n = hi - lo;
+        it.first = first;
+        it.last = last;
       }
       const int slot = wave % kItems;
       ok = wait_bar_short(item_empty(slot), ((wave / kItems) & 1) ^ 1, ctl, 510);
@@ -559,19 +562,22 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
         return true;
       };
+      auto zero_rows = [&](unsigned char* v, int from, int to) {
+#pragma unroll 1
+        for (int e = from * 8 + lane; e < to * 8; e += 32)
+#pragma unroll
+          for (int c = 0; c < C::kChunks; ++c) *reinterpret_cast<uint4*>(v + c * (kKeys * 128) + e * 16) = make_uint4(0, 0, 0, 0);
+      };
       auto product = [&](int i, int j) {  // O += P V of step i
         if (i < 0) return true;
         const int tt = t0 + j;
-        // value rows past the sequence's last key belong to someone else: 0 * anything finite or not must be 0
-        // (with two MMA warps both write these zeros)
-        const int valid = it.kn - (it.lo + i) * kKeys;
-        if (!PREFIX && j == 0 && valid < kKeys) {
+        // Value rows that no row of the item sees (other sequences' rows, later and windowed-out keys) become zeros: a weight
+        // of 0 times what is there must be 0, finite or not.  (With two MMA warps both write the zeros.)
+        const int key = (it.lo + i) * kKeys, head = min(it.first - key, kKeys), tail = it.last + 1 - key;
+        if (j == 0 && (head > 0 || tail < kKeys)) {
           unsigned char* v = smem + C::OFF_KV + (2 * cv + 1) * C::kTile;
-#pragma unroll 1
-          for (int e = valid * 8 + lane; e < kKeys * 8; e += 32)
-#pragma unroll
-            for (int c = 0; c < C::kChunks; ++c)
-              *reinterpret_cast<uint4*>(v + c * (kKeys * 128) + e * 16) = make_uint4(0, 0, 0, 0);
+          if (head > 0) zero_rows(v, 0, head);
+          if (tail < kKeys) zero_rows(v, tail, kKeys);
           fence_proxy_async();
           __syncwarp();
         }

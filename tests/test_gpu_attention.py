@@ -168,6 +168,34 @@ def test_prompt_neighbours_do_not_reach_a_sequence(d, bad):
     assert got[:70].isnan().any()
 
 
+@pytest.mark.parametrize("d,heads", [(64, 8), (128, 1)])
+@pytest.mark.parametrize("lq,lk,window", [([40], [500], 64), ([5, 300], [200, 700], 30), ([1, 1], [129, 127], 1)])
+def test_prompt_keys_that_no_row_sees_may_hold_anything(d, heads, lq, lk, window):
+    """Keys before every row's window (dropped by a cache, say) hold not-a-numbers."""
+    from kcapw_klcquant_b200 import attn_prompt
+
+    q, k, v = rnd((sum(lq), heads, d), BF, 9), rnd((sum(lk), 1, d), BF, 10), rnd((sum(lk), 1, d), BF, 11)
+    clean = attn_prompt(q, k, v, cum(lq), cu_seqlens_k=cum(lk), window=window)
+    check_prompt(q, k, v, lq, lk, window, None, clean, None, d ** -0.5)
+    at = 0
+    for n, m in zip(lq, lk):
+        k[at:at + m - n - window + 1] = float("nan")
+        v[at:at + m - n - window + 1] = float("inf")
+        at += m
+    assert torch.equal(attn_prompt(q, k, v, cum(lq), cu_seqlens_k=cum(lk), window=window), clean)
+
+
+def test_prompt_later_values_do_not_reach_earlier_row_tiles():
+    """A value that is not finite reaches rows from its own on, and at most the rows of its own two row tiles before it."""
+    from kcapw_klcquant_b200 import attn_prompt
+
+    q, k, v = rnd((400, 16, 64), BF, 12), rnd((400, 2, 64), BF, 13), rnd((400, 2, 64), BF, 14)
+    clean = attn_prompt(q, k, v, cum([400]))
+    v[200] = float("nan")
+    got = attn_prompt(q, k, v, cum([400]))
+    assert got[200:].isnan().all() and torch.equal(got[:192], clean[:192])  # 8 heads a key head: 16 tokens a row tile
+
+
 def test_prompt_nan_key_is_a_nan_row():
     from kcapw_klcquant_b200 import attn_prompt
 
