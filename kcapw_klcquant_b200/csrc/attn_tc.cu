@@ -75,6 +75,7 @@ constexpr int kKeys = 128;     // keys of a key tile
 constexpr int kThreads = 352;  // 8 softmax warps, an MMA warp for each row tile, TMA warp
 constexpr int kSoftmaxWarps = 8, kWarpMma0 = 8, kWarpTma = 9, kWarpMma1 = 10;
 constexpr uint32_t kTmemCols = 512;
+constexpr int kOutPitch = 80, kOutWarp = 32 * kOutPitch;
 constexpr float kRescaleLog2 = 8.f;
 constexpr int kItems = 2;      // ring of items between the TMA warp and the others
 
@@ -266,7 +267,8 @@ struct Cfg {
   static constexpr int kBars = 2 * kStages + 2 + 10 + 2 * kItems + 1;
   static constexpr int OFF_MISC = OFF_BAR + kBars * 8;
   static constexpr int OFF_ITEM = OFF_MISC + 16;
-  static constexpr int kSmem = OFF_ITEM + kItems * int(sizeof(Item)) + 1024;  // + alignment of the swizzled tiles
+  static constexpr int OFF_OUT = (OFF_ITEM + kItems * int(sizeof(Item)) + 15) / 16 * 16;  // per softmax warp: 32 rows of 64 + 16 bytes
+  static constexpr int kSmem = OFF_OUT + kSoftmaxWarps * kOutWarp + 1024;  // + alignment of the swizzled tiles
 };
 
 // ---------------------------------------------------------------------------
@@ -832,8 +834,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           finish_row(m, l, p.sinks != nullptr, sink, &inv, &lse);
           if (p.lse != nullptr) p.lse[row * p.heads + head] = lse;
         }
-        uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + row * p.out_ts + int64_t(head) * p.out_hs);
+        // D = 128: through shared memory, 32 columns at a time, so that four lanes store 64 bytes of a row (1106 against 1067
+        // TFLOP/s at 6016 tokens); D = 64: straight from the rows' threads (718 against 678).
+        constexpr bool kStaged = D == 128;
+        const int64_t mine = row_ok ? row * p.out_ts + int64_t(head) * p.out_hs : -1;
+        int64_t off[4];  // of the rows this lane stores: 8 k + lane / 4 of the warp's
+        unsigned char* stage = smem + C::OFF_OUT + warp * kOutWarp;
+        if constexpr (kStaged) {
 #pragma unroll
+          for (int k = 0; k < 4; ++k) off[k] = __shfl_sync(0xffffffffu, mine, 8 * k + (lane >> 2));
+        }
+#pragma unroll(kStaged ? 1 : 2)
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
           if (it.n > 0) {
@@ -843,16 +854,25 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = 0.f;
           }
-          if (row_ok) {
+          T* out = reinterpret_cast<T*>(p.out) + 32 * c;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint4 w;
-              w.x = Elem<T>::pack(o[8 * j] * inv, o[8 * j + 1] * inv);
-              w.y = Elem<T>::pack(o[8 * j + 2] * inv, o[8 * j + 3] * inv);
-              w.z = Elem<T>::pack(o[8 * j + 4] * inv, o[8 * j + 5] * inv);
-              w.w = Elem<T>::pack(o[8 * j + 6] * inv, o[8 * j + 7] * inv);
-              dst[c * 4 + j] = w;
+          for (int j = 0; j < 4; ++j) {
+            uint4 w;
+            w.x = Elem<T>::pack(o[8 * j] * inv, o[8 * j + 1] * inv);
+            w.y = Elem<T>::pack(o[8 * j + 2] * inv, o[8 * j + 3] * inv);
+            w.z = Elem<T>::pack(o[8 * j + 4] * inv, o[8 * j + 5] * inv);
+            w.w = Elem<T>::pack(o[8 * j + 6] * inv, o[8 * j + 7] * inv);
+            if constexpr (kStaged) *reinterpret_cast<uint4*>(stage + lane * kOutPitch + 16 * j) = w;
+            else if (row_ok) *reinterpret_cast<uint4*>(out + mine + 8 * j) = w;
+          }
+          __syncwarp();
+          if constexpr (kStaged) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint4 w = *reinterpret_cast<const uint4*>(stage + (8 * k + (lane >> 2)) * kOutPitch + (lane & 3) * 16);
+              if (off[k] >= 0) *reinterpret_cast<uint4*>(out + off[k] + (lane & 3) * 8) = w;
             }
+            __syncwarp();
           }
         }
       }
