@@ -836,17 +836,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
         // D = 128: through shared memory, 32 columns at a time, so that four lanes store 64 bytes of a row (1106 against 1067
         // TFLOP/s at 6016 tokens); D = 64: straight from the rows' threads (718 against 678).
-        constexpr bool kStaged = D == 128;
-        const int64_t mine = row_ok ? row * p.out_ts + int64_t(head) * p.out_hs : -1;
-        int64_t off[4];  // of the rows this lane stores: 8 k + lane / 4 of the warp's
-        unsigned char* stage = smem + C::OFF_OUT + warp * kOutWarp;
-        if constexpr (kStaged) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) off[k] = __shfl_sync(0xffffffffu, mine, 8 * k + (lane >> 2));
-        }
-#pragma unroll(kStaged ? 1 : 2)
-        for (int c = 0; c < D / 32; ++c) {
-          float o[32];
+        auto columns = [&](int c, float* o) {  // 32 columns of O
           if (it.n > 0) {
             tmem_ld32(o_col + uint32_t(32 * c), o);
             tmem_wait_ld32(o);
@@ -854,25 +844,45 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = 0.f;
           }
-          T* out = reinterpret_cast<T*>(p.out) + 32 * c;
+        };
+        auto packed = [&](const float* o, int j) {  // eight of them, finished
+          uint4 w;
+          w.x = Elem<T>::pack(o[8 * j] * inv, o[8 * j + 1] * inv);
+          w.y = Elem<T>::pack(o[8 * j + 2] * inv, o[8 * j + 3] * inv);
+          w.z = Elem<T>::pack(o[8 * j + 4] * inv, o[8 * j + 5] * inv);
+          w.w = Elem<T>::pack(o[8 * j + 6] * inv, o[8 * j + 7] * inv);
+          return w;
+        };
+        if constexpr (D == 128) {
+          const int64_t mine = row_ok ? row * p.out_ts + int64_t(head) * p.out_hs : -1;
+          int64_t off[4];  // of the rows this lane stores: 8 k + lane / 4 of the warp's
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint4 w;
-            w.x = Elem<T>::pack(o[8 * j] * inv, o[8 * j + 1] * inv);
-            w.y = Elem<T>::pack(o[8 * j + 2] * inv, o[8 * j + 3] * inv);
-            w.z = Elem<T>::pack(o[8 * j + 4] * inv, o[8 * j + 5] * inv);
-            w.w = Elem<T>::pack(o[8 * j + 6] * inv, o[8 * j + 7] * inv);
-            if constexpr (kStaged) *reinterpret_cast<uint4*>(stage + lane * kOutPitch + 16 * j) = w;
-            else if (row_ok) *reinterpret_cast<uint4*>(out + mine + 8 * j) = w;
-          }
-          __syncwarp();
-          if constexpr (kStaged) {
+          for (int k = 0; k < 4; ++k) off[k] = __shfl_sync(0xffffffffu, mine, 8 * k + (lane >> 2));
+          unsigned char* stage = smem + C::OFF_OUT + warp * kOutWarp;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            columns(c, o);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage + lane * kOutPitch + 16 * j) = packed(o, j);
+            __syncwarp();
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const uint4 w = *reinterpret_cast<const uint4*>(stage + (8 * k + (lane >> 2)) * kOutPitch + (lane & 3) * 16);
-              if (off[k] >= 0) *reinterpret_cast<uint4*>(out + off[k] + (lane & 3) * 8) = w;
+              if (off[k] >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + off[k] + 32 * c + (lane & 3) * 8) = w;
             }
             __syncwarp();
+          }
+        } else {
+          uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + row * p.out_ts + int64_t(head) * p.out_hs);
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            columns(c, o);
+            if (row_ok) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) dst[c * 4 + j] = packed(o, j);
+            }
           }
         }
       }
