@@ -121,7 +121,8 @@ def _dims(q: torch.Tensor, kv_heads: int, window: int, scale: float | None) -> _
 
 def _out(out: torch.Tensor | None, q: torch.Tensor, index: int) -> tuple[torch.Tensor, int, int, int]:
     if out is None:
-        out = q.new_empty(q.shape)
+        # (empty_like costs half of empty, and is contiguous unless heads lie outside tokens)
+        out = torch.empty_like(q) if q.stride(0) >= q.stride(1) else q.new_empty(q.shape)
     elif out.shape != q.shape:
         raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
     got = _rows("out", out, q.dtype, index)

@@ -193,7 +193,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     prefetch_map(&map_v);
   }
   pdl_trigger();
-  if (!p.after_prefix) pdl_wait();  // behind the prefix kernel, its inputs are complete already
+  if (!p.after_prefix) pdl_wait();  // started by the prefix kernel, which has waited for what came before
 
   // ---- prefix sums of the sequences' tiles
   const int per = (p.batch + kThreads - 1) / kThreads, b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
@@ -470,6 +470,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const DecodeParams p, int ctas) {
   constexpr int V = D / 32;  // values a lane
   pdl_wait();
+  pdl_trigger();
   const int lane = threadIdx.x & 31;
   const int64_t rid = int64_t(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5);
   if (rid >= int64_t(p.batch) * p.heads) return;

@@ -332,7 +332,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (PREFIX) pdl_trigger();  // the decode kernel may run beside this one
   if (warp == kWarpMma0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
                  "r"(kTmemCols));
@@ -342,6 +341,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_holder, 0);
+  pdl_wait();     // set up under the previous kernel's tail; from here on its results are read
+  pdl_trigger();  // the next kernel may set up meanwhile (prefix: the decode kernel may run beside this one)
 
   // the next item of the ring for a consumer warp; false after the last one or on an abort
   uint32_t item_no = 0;
@@ -902,7 +903,7 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
   static SmemLimit limit;
   int st = limit.raise(reinterpret_cast<const void*>(kernel), Cfg<D>::kSmem);
   if (st != KLC_OK) return st;
-  kernel<<<unsigned(std::min<int64_t>(items, sm_count())), kThreads, Cfg<D>::kSmem, s>>>(mq, mk, mv, p);
+  KLC_CUDA(launch_chain(kernel, dim3(unsigned(std::min<int64_t>(items, sm_count()))), dim3(kThreads), Cfg<D>::kSmem, s, 0, mq, mk, mv, p));
   KLC_LAUNCH_CHECK(PREFIX ? "attn_prefix" : "attn_prompt");
   return KLC_OK;
 }
