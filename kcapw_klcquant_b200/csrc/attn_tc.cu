@@ -242,7 +242,7 @@ struct Item {
   int k0, kn;  // first key row and number of keys
   int tok0;    // first token of the item's row tiles; -1: no more items
   int tiles;   // row tiles with rows: 1 or 2
-  int lo, n;   // key tiles lo .. lo + n
+  int lo, n;   // first key of the item's tiles, and their number
   int kvh, z;  // key head; prefix: share of the keys
   int first, last;  // lowest and highest key that some row of the item sees
 };
@@ -268,7 +268,7 @@ struct Cfg {
   static constexpr int OFF_MISC = OFF_BAR + kBars * 8;
   static constexpr int OFF_ITEM = OFF_MISC + 16;
   static constexpr int OFF_OUT = (OFF_ITEM + kItems * int(sizeof(Item)) + 15) / 16 * 16;  // per softmax warp: 32 rows of 64 + 16 bytes
-  static constexpr int kSmem = OFF_OUT + kSoftmaxWarps * kOutWarp + 1024;  // + alignment of the swizzled tiles
+  static constexpr int kSmem = OFF_OUT + (D == 128 ? kSoftmaxWarps * kOutWarp : 0) + 1024;  // + alignment of the swizzled tiles
 };
 
 // ---------------------------------------------------------------------------
@@ -433,15 +433,16 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
           last = it.kn - it.qn + min(it.tok0 + 2 * tpt, it.qn) - 1;
         }
-        int lo = 0, hi = 0;
-        if (last >= first) lo = first / kKeys, hi = last / kKeys + 1;
-        if (PREFIX) {  // this item's share of the keys
-          const int n = hi - lo;
-          hi = lo + int(int64_t(n) * (it.z + 1) / p.splits);
-          lo = lo + int(int64_t(n) * it.z / p.splits);
+        if (PREFIX) {  // this item's share of the tiles, which start where pages do
+          int lo = 0, n = 0;
+          if (last >= first) lo = first / kKeys, n = last / kKeys + 1 - lo;
+          const int a = int(int64_t(n) * it.z / p.splits);
+          it.lo = (lo + a) * kKeys;
+          it.n = int(int64_t(n) * (it.z + 1) / p.splits) - a;
+        } else if (last >= first) {
+          it.lo = first;
+          it.n = (last - first) / kKeys + 1;
         }
-        it.lo = lo;
-        it.n = hi - lo;
         it.first = first;
         it.last = last;
       }
@@ -455,7 +456,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       if (it.tok0 < 0) break;
       if (lane == 0) {
         for (int i = 0; i < it.n; ++i, ++issued) {
-          const int key = (it.lo + i) * kKeys, s = issued % C::kStages;
+          const int key = it.lo + i * kKeys, s = issued % C::kStages;
           if (!(ok = wait_bar_short(kv_empty(s), ((issued / C::kStages) & 1) ^ 1, ctl, 501))) break;
           mbar_arrive_expect_tx(kv_full(s), 2u * uint32_t(C::kTile));
           for (int kv = 0; kv < 2; ++kv) {
@@ -576,7 +577,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         const int tt = t0 + j;
         // Value rows that no row of the item sees (other sequences' rows, later and windowed-out keys) become zeros: a weight
         // of 0 times what is there must be 0, finite or not.  (With two MMA warps both write the zeros.)
-        const int key = (it.lo + i) * kKeys, head = min(it.first - key, kKeys), tail = it.last + 1 - key;
+        const int key = it.lo + i * kKeys, head = min(it.first - key, kKeys), tail = it.last + 1 - key;
         if (j == 0 && (head > 0 || tail < kKeys)) {
           unsigned char* v = smem + C::OFF_KV + (2 * cv + 1) * C::kTile;
           if (head > 0) zero_rows(v, 0, head);
@@ -660,7 +661,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         ok = wait_bar_short(s_full(t), steps & 1, ctl, 508);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
-        const int kb = (it.lo + i) * kKeys;
+        const int kb = it.lo + i * kKeys;
         const bool masked = kb < wlo || kb + kKeys - 1 > whi;
         const int ja = jlo - kb, jb = jhi - kb;
         // Columns 0-63 are read twice and 64-127 kept (all 128 would not fit the registers).
@@ -837,23 +838,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
         // D = 128: through shared memory, 32 columns at a time, so that four lanes store 64 bytes of a row (1106 against 1067
         // TFLOP/s at 6016 tokens); D = 64: straight from the rows' threads (718 against 678).
-        auto columns = [&](int c, float* o) {  // 32 columns of O
-          if (it.n > 0) {
-            tmem_ld32(o_col + uint32_t(32 * c), o);
-            tmem_wait_ld32(o);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = 0.f;
-          }
-        };
-        auto packed = [&](const float* o, int j) {  // eight of them, finished
-          uint4 w;
-          w.x = Elem<T>::pack(o[8 * j] * inv, o[8 * j + 1] * inv);
-          w.y = Elem<T>::pack(o[8 * j + 2] * inv, o[8 * j + 3] * inv);
-          w.z = Elem<T>::pack(o[8 * j + 4] * inv, o[8 * j + 5] * inv);
-          w.w = Elem<T>::pack(o[8 * j + 6] * inv, o[8 * j + 7] * inv);
-          return w;
-        };
         if constexpr (D == 128) {
           const int64_t mine = row_ok ? row * p.out_ts + int64_t(head) * p.out_hs : -1;
           int64_t off[4];  // of the rows this lane stores: 8 k + lane / 4 of the warp's
@@ -863,9 +847,22 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             float o[32];
-            columns(c, o);
+            if (it.n > 0) {
+              tmem_ld32(o_col + uint32_t(32 * c), o);
+              tmem_wait_ld32(o);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage + lane * kOutPitch + 16 * j) = packed(o, j);
+              for (int j = 0; j < 32; ++j) o[j] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint4 w;
+              w.x = Elem<T>::pack(o[8 * j] * inv, o[8 * j + 1] * inv);
+              w.y = Elem<T>::pack(o[8 * j + 2] * inv, o[8 * j + 3] * inv);
+              w.z = Elem<T>::pack(o[8 * j + 4] * inv, o[8 * j + 5] * inv);
+              w.w = Elem<T>::pack(o[8 * j + 6] * inv, o[8 * j + 7] * inv);
+              *reinterpret_cast<uint4*>(stage + lane * kOutPitch + 16 * j) = w;
+            }
             __syncwarp();
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -879,10 +876,23 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             float o[32];
-            columns(c, o);
+            if (it.n > 0) {
+              tmem_ld32(o_col + uint32_t(32 * c), o);
+              tmem_wait_ld32(o);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = 0.f;
+            }
             if (row_ok) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) dst[c * 4 + j] = packed(o, j);
+              for (int j = 0; j < 4; ++j) {
+                uint4 w;
+                w.x = Elem<T>::pack(o[8 * j] * inv, o[8 * j + 1] * inv);
+                w.y = Elem<T>::pack(o[8 * j + 2] * inv, o[8 * j + 3] * inv);
+                w.z = Elem<T>::pack(o[8 * j + 4] * inv, o[8 * j + 5] * inv);
+                w.w = Elem<T>::pack(o[8 * j + 6] * inv, o[8 * j + 7] * inv);
+                dst[c * 4 + j] = w;
+              }
             }
           }
         }
