@@ -24,7 +24,7 @@ import threading
 import torch
 
 from . import _lib
-from .moe import as_bf16, workspace
+from .moe import _WORKSPACES, as_bf16, workspace
 
 # the current stream of a device as an integer, without making a Stream object for it where torch offers that
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _lib.stream_ptr)
@@ -109,6 +109,11 @@ def _sinks(sinks: torch.Tensor | None, heads: int, index: int) -> torch.Tensor |
     return sinks if sinks.is_contiguous() else sinks.contiguous()
 
 
+@functools.lru_cache(maxsize=256)
+def _dims_of(code: int, heads: int, kv_heads: int, d: int, window: int, scale: float) -> _lib.KlcAttnDims:
+    return _lib.KlcAttnDims(code, heads, kv_heads, d, window, scale)
+
+
 def _dims(q: torch.Tensor, kv_heads: int, window: int, scale: float | None) -> _lib.KlcAttnDims:
     code = _lib.DTYPE_CODE.get(q.dtype)
     if code is None or q.dtype is torch.float32:
@@ -116,14 +121,17 @@ def _dims(q: torch.Tensor, kv_heads: int, window: int, scale: float | None) -> _
     if not 0 <= window < 1 << 31:
         raise ValueError("window must be >= 0 and fit 32 bits")
     _, heads, d = q.shape
-    return _lib.KlcAttnDims(code, heads, kv_heads, d, window, d ** -0.5 if scale is None else scale)
+    return _dims_of(code, heads, kv_heads, d, window, d ** -0.5 if scale is None else float(scale))
 
 
 def _out(out: torch.Tensor | None, q: torch.Tensor, index: int) -> tuple[torch.Tensor, int, int, int]:
     if out is None:
-        # (empty_like costs half of empty, and is contiguous unless heads lie outside tokens)
-        out = torch.empty_like(q) if q.stride(0) >= q.stride(1) else q.new_empty(q.shape)
-    elif out.shape != q.shape:
+        out = torch.empty_like(q)  # (half the time of empty; contiguous unless q's heads lie outside its tokens)
+        if not out.is_contiguous():
+            out = q.new_empty(q.shape)
+        _, h, d = q.shape
+        return out, out.data_ptr(), h * d, d
+    if out.shape != q.shape:
         raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
     got = _rows("out", out, q.dtype, index)
     if got[0] is not out:
@@ -223,7 +231,8 @@ def _workspace(device: torch.device, nbytes: int, stream: int) -> torch.Tensor:
     graphs never share it, on whichever streams they are replayed)."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return workspace(device, nbytes, stream)
+    ws = _WORKSPACES.get((device.index, stream))
+    return ws if ws is not None and ws.numel() >= nbytes else workspace(device, nbytes, stream)
 
 
 def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype, index: int, d: int) -> tuple[int, int]:
