@@ -23,9 +23,9 @@
 //
 // Bound: with D = 128 the chain softmax -> P V -> next S of a row tile (TMEM
 // has no room for a second S), with D = 64 the softmax's instructions.  16221
-// tokens, 32 / 8 heads of 128: 2.04 ms, 1.06 PFLOP/s, 62 % of the burst rate of
-// a library product (73 % of its sustained one); 6016 tokens, 64 / 8 heads of
-// 64: 410 us, 725 TFLOP/s.
+// tokens, 32 / 8 heads of 128: 1.98 ms, 1.09 PFLOP/s, 63 % of the burst rate of
+// a library product (75 % of its sustained one); 6016 tokens, 64 / 8 heads of
+// 64: 404 us, 735 TFLOP/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -671,7 +671,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         tmem_wait_ld64(sa);
         tmem_ld64(s_col + 64, sb);
         // boundary tiles, 32 columns at a time: bit c, no row of the warp sees any / some row does not see all of columns 32 c ..
-        // (D = 64: 2 to 6 % on ragged and windowed prompts; with D = 128 it cost 2 % in registers)
+        // (D = 64: 2 to 6 % faster on ragged and windowed prompts; with D = 128 2 % slower, by registers)
         uint32_t none = 0, part = masked ? 15u : 0u;
         if (C::kOwnP && masked) {
           part = 0;
