@@ -467,11 +467,8 @@ int klc_status_bytes(size_t* out_bytes);
  * key: with more keys than queries the first keys are an earlier part of the
  * sequence.  Token and head strides are in elements, multiples of 8; rows are
  * 16-byte aligned.  lse fp32 [q_tokens, heads] or NULL.  Rows of out past
- * cu_q[batch] are not written; out may be q.  Keys and values that no row
- * sees (padding, other sequences' rows, keys before every window) may hold
- * anything.  A value of the sequence's own that is not finite reaches the rows
- * that see it and may reach the others of their 256 / G neighbouring tokens (G
- * query heads per key head).  Offsets that leave the tensors are recorded as
+ * cu_q[batch] are not written; out may be q.  A key or value reaches the
+ * rows that see it and no others, whatever it holds.  Offsets that leave the tensors are recorded as
  * KLC_ERR_DEVICE_FAULT and the sequence is skipped.  Replaces StreamedAttention.forward's loop over the tokens of a
  * prompt. */
 int klc_attn_prompt(const klc_attn_dims* dims, const void* q, int64_t q_tokens, int64_t q_token_stride,
@@ -491,8 +488,7 @@ int klc_attn_prompt(const klc_attn_dims* dims, const void* q, int64_t q_tokens, 
  * group_starts[g] .. group_starts[g+1] (int32 on the device, ascending), whose
  * first prefix_lens[g] keys (a multiple of page_size) are the same pages: they
  * are read once for the whole group, through the table of its first row; rows
- * outside the groups have none.  (A prefix value that is not finite may reach
- * every row of its group, a window or not.)
+ * outside the groups have none.
  * The split over SMs is made on the device from lens, so a captured call
  * serves other lengths on replay.  Results do not depend on timing.  A page id
  * outside [0, pages) and a length outside [0, table_width * page_size] are

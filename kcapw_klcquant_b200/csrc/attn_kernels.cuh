@@ -22,6 +22,8 @@ struct TcParams {
   int64_t out_ts, out_hs;
   float* lse;
   DeviceStatus* status;
+  const void* v;       // values, for elements that are not finite: token and head stride (prompts), page stride (v_ts, prefix)
+  int64_t v_ts, v_hs;
   // prefix of decode rows
   const int32_t* prefix_lens;  // [batch]
   const int32_t* lens;         // [total_q]

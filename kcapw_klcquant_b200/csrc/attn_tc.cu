@@ -11,7 +11,7 @@
 // sequences fill tiles that 128 tokens of one head would not.  Keys come in
 // tiles of 128.  Warps:
 //   0-3, 4-7  softmax of row tile 0 / 1, one row per thread (TMEM lane = row)
-//   8, 10     MMA issuer of row tile 0 / 1 (one thread); zeroes value rows that no row of the item sees
+//   8, 10     MMA issuer of row tile 0 / 1 (one thread); settles values that not all rows of the item see
 //   9         finds the items; TMA producer (queries, then a ring of key and value tiles)
 // Per key tile and row tile: S = Q K^T into TMEM (128 fp32 columns), the
 // softmax thread reads its row and writes P as 16-bit pairs, and O += P V
@@ -23,9 +23,9 @@
 //
 // Bound: with D = 128 the chain softmax -> P V -> next S of a row tile (TMEM
 // has no room for a second S), with D = 64 the softmax's instructions.  16221
-// tokens, 32 / 8 heads of 128: 1.98 ms, 1.09 PFLOP/s, 63 % of the burst rate of
-// a library product (75 % of its sustained one); 6016 tokens, 64 / 8 heads of
-// 64: 404 us, 735 TFLOP/s.
+// tokens, 32 / 8 heads of 128: 2.04 ms, 1.06 PFLOP/s, 62 % of the burst rate of
+// a library product (73 % of its sustained one); 6016 tokens, 64 / 8 heads of
+// 64: 408 us, 727 TFLOP/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -237,6 +237,64 @@ __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t mn_stride) 
   return ((saddr & 0x3FFFFu) >> 4) | ((mn_stride == 0 ? 1u : mn_stride >> 4) << 16);
 }
 
+// Whether this lane's share of the rows [from, to) of a value tile holds an element that is not finite; with CLEAR, these
+// become 0.
+template <typename T, int CHUNKS, bool CLEAR>
+__device__ bool odd_rows(unsigned char* v, int from, int to, int lane) {
+  constexpr uint32_t kExp = Elem<T>::kMmaFormat == 1 ? 0x7f80u : 0x7c00u;  // all ones: infinite or not a number
+  bool some = false;
+#pragma unroll 1
+  for (int e = from * 8 + lane; e < to * 8; e += 32)
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      uint4* at = reinterpret_cast<uint4*>(v + c * (kKeys * 128) + e * 16);
+      uint4 x = *at;
+      uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool lo = (w[i] & kExp) == kExp, hi = ((w[i] >> 16) & kExp) == kExp;
+        some |= lo | hi;
+        if (CLEAR) w[i] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
+      }
+      if (CLEAR) *at = x;
+    }
+  return some;
+}
+
+// A value tile whose keys [0, 128) not all rows of the item see, before its product: [first, end) are seen by some row,
+// [all_lo, all_end) by all.  A masked weight is 0, and 0 times what is stored must be 0, finite or not:
+//   * rows that nobody sees (other sequences', later, windowed out) become zeros;
+//   * in rows that some see, elements that are not finite become zeros; `mark` gets `number`, and the rows that see them add them
+//     back at the end (add_odd).
+// Out of line: it runs on few tiles, and the MMA warp's code is to stay small.  (With two MMA warps both do this, with the same
+// result; the mark is there before an element is gone for the other.)
+template <typename T, int CHUNKS>
+__device__ __noinline__ void settle_values(unsigned char* v, int first, int end, int all_lo, int all_end, volatile uint32_t* mark,
+                                           uint32_t number) {
+  const int lane = threadIdx.x & 31;
+  first = min(max(first, 0), kKeys);
+  end = max(min(end, kKeys), first);
+  auto zero = [&](int from, int to) {
+#pragma unroll 1
+    for (int e = from * 8 + lane; e < to * 8; e += 32)
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) *reinterpret_cast<uint4*>(v + c * (kKeys * 128) + e * 16) = make_uint4(0, 0, 0, 0);
+  };
+  zero(0, first);
+  zero(end, kKeys);
+  const int a1 = min(all_lo, end), b0 = max(all_end, first);
+  const bool some = odd_rows<T, CHUNKS, false>(v, first, a1, lane) | odd_rows<T, CHUNKS, false>(v, b0, end, lane);
+  if (__any_sync(0xffffffffu, some)) {
+    if (lane == 0) *mark = number;
+    __threadfence_block();
+    __syncwarp();
+    odd_rows<T, CHUNKS, true>(v, first, a1, lane);
+    odd_rows<T, CHUNKS, true>(v, b0, end, lane);
+  }
+  fence_proxy_async();
+  __syncwarp();
+}
+
 struct Item {
   int q0, qn;  // the sequence's first query row and its number of query rows (tokens)
   int k0, kn;  // first key row and number of keys
@@ -245,6 +303,7 @@ struct Item {
   int lo, n;   // first key of the item's tiles, and their number
   int kvh, z;  // key head; prefix: share of the keys
   int first, last;  // lowest and highest key that some row of the item sees
+  int all_lo, all_hi;  // every row sees the keys from all_lo to all_hi
 };
 
 template <int D>
@@ -266,10 +325,45 @@ struct Cfg {
   static constexpr int OFF_BAR = OFF_KV + kStages * 2 * kTile;
   static constexpr int kBars = 2 * kStages + 2 + 10 + 2 * kItems + 1;
   static constexpr int OFF_MISC = OFF_BAR + kBars * 8;
-  static constexpr int OFF_ITEM = OFF_MISC + 16;
-  static constexpr int OFF_OUT = (OFF_ITEM + kItems * int(sizeof(Item)) + 15) / 16 * 16;  // per softmax warp: 32 rows of 64 + 16 bytes
+  static constexpr int OFF_ITEM = OFF_MISC + 32;
+  static constexpr int OFF_RECENT = OFF_ITEM + kItems * int(sizeof(Item));  // the last four items
+  static constexpr int OFF_OUT = (OFF_RECENT + 4 * int(sizeof(Item)) + 15) / 16 * 16;  // per softmax warp: 32 rows of 64 + 16 bytes
   static constexpr int kSmem = OFF_OUT + (D == 128 ? kSoftmaxWarps * kOutWarp : 0) + 1024;  // + alignment of the swizzled tiles
 };
+
+// Adds to a row's output in TMEM what odd_rows took out of the values: the elements that are not finite of those keys that the
+// row, but not every row of the item, sees (a positive weight times an infinity or a NaN is that).
+template <typename T, int D, bool PREFIX>
+__device__ __noinline__ void add_odd(uint32_t o_col, const Item& it, const TcParams& p, int jlo, int jhi) {
+  for (int c = 0; c < D / 32; ++c) {
+    float o[32];
+    tmem_ld32(o_col + uint32_t(32 * c), o);
+    tmem_wait_ld32(o);
+    for (int j = max(it.first, jlo); j <= min(it.last, jhi); ++j) {
+      if (j >= it.all_lo && j <= it.all_hi) {
+        j = it.all_hi;
+        continue;
+      }
+      const T* v = reinterpret_cast<const T*>(p.v) + 32 * c;
+      if (PREFIX) {
+        const int page = p.block_table[int64_t(it.q0) * p.table_stride + j / p.page_size];
+        if (page < 0 || page >= p.pages) continue;
+        v += page * p.v_ts + (int64_t(it.kvh) * p.page_size + j % p.page_size) * D;
+      } else {
+        v += (int64_t(it.k0) + j) * p.v_ts + int64_t(it.kvh) * p.v_hs;
+      }
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        const float2 x = Elem<T>::unpack(*reinterpret_cast<const uint32_t*>(v + e));
+        if (!isfinite(x.x)) o[e] += x.x;
+        if (!isfinite(x.y)) o[e + 1] += x.y;
+      }
+    }
+    __syncwarp();
+    tmem_st32(o_col + uint32_t(32 * c), reinterpret_cast<const uint32_t*>(o));
+  }
+  tmem_wait_st();
+}
 
 // ---------------------------------------------------------------------------
 // PREFIX = false: packed prompts.  PREFIX = true: single-token rows over the pages of their group's prefix, keys
@@ -282,7 +376,7 @@ struct Cfg {
 template <typename T, int D, bool PREFIX>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-               const __grid_constant__ CUtensorMap map_v, const TcParams p) {
+               const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcParams p) {
   using C = Cfg<D>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -304,6 +398,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const uint32_t mma_done = bar0 + 8u * (kB + 12 + 2 * kItems);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
+  // [4]: number of the last item (+ 1, by item number mod 4) in which a value that only some rows see was not finite
+  volatile uint32_t* odd = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_MISC + 8);
+  Item* recent = reinterpret_cast<Item*>(smem + C::OFF_RECENT);
   Item* items = reinterpret_cast<Item*>(smem + C::OFF_ITEM);
   const Ctl ctl{abort_flag, p.status};
 
@@ -330,6 +427,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     }
     mbar_init(mma_done, C::kMmaWarps);
     *abort_flag = 0;
+    for (int i = 0; i < 4; ++i) odd[i] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kWarpMma0) {
@@ -368,7 +466,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       const int64_t idx = int64_t(wave) * gridDim.x + ((wave & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
       const int64_t pair = idx / unit;
       const int sub = int(idx - pair * unit);
-      Item it{0, 0, 0, 0, -1, 0, 0, 0, 0, 0, 0, 0};
+      Item it{0, 0, 0, 0, -1, 0, 0, 0, 0, 0, 0, 0, 0, 0};
       for (; seq0 < p.batch; seq0 += 32) {
         const int s = seq0 + lane;
         int qb = 0, qn = 0, kb = 0, kn = 0;
@@ -428,10 +526,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           hi = __reduce_max_sync(0xffffffffu, hi);
           first = p.window > 0 ? max(0, lo - p.window) : 0;
           last = min(hi, it.kn) - 1;
+          it.all_lo = p.window > 0 ? max(0, hi - p.window) : 0;
+          it.all_hi = min(lo, it.kn) - 1;
         } else {
           const int pos = it.kn - it.qn + it.tok0;
           first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
           last = it.kn - it.qn + min(it.tok0 + 2 * tpt, it.qn) - 1;
+          it.all_lo = p.window > 0 ? max(0, last - p.window + 1) : 0;
+          it.all_hi = pos;
         }
         if (PREFIX) {  // this item's share of the tiles, which start where pages do
           int lo = 0, n = 0;
@@ -451,6 +553,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       if (lane == 0) {
         items[slot] = it;
+        recent[wave & 3] = it;
         mbar_arrive(item_full(slot));
       }
       if (it.tok0 < 0) break;
@@ -566,24 +669,13 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
         return true;
       };
-      auto zero_rows = [&](unsigned char* v, int from, int to) {
-#pragma unroll 1
-        for (int e = from * 8 + lane; e < to * 8; e += 32)
-#pragma unroll
-          for (int c = 0; c < C::kChunks; ++c) *reinterpret_cast<uint4*>(v + c * (kKeys * 128) + e * 16) = make_uint4(0, 0, 0, 0);
-      };
       auto product = [&](int i, int j) {  // O += P V of step i
         if (i < 0) return true;
         const int tt = t0 + j;
-        // Value rows that no row of the item sees (other sequences' rows, later and windowed-out keys) become zeros: a weight
-        // of 0 times what is there must be 0, finite or not.  (With two MMA warps both write the zeros.)
-        const int key = it.lo + i * kKeys, head = min(it.first - key, kKeys), tail = it.last + 1 - key;
-        if (j == 0 && (head > 0 || tail < kKeys)) {
-          unsigned char* v = smem + C::OFF_KV + (2 * cv + 1) * C::kTile;
-          if (head > 0) zero_rows(v, 0, head);
-          if (tail < kKeys) zero_rows(v, tail, kKeys);
-          fence_proxy_async();
-          __syncwarp();
+        const int key = it.lo + i * kKeys;
+        if (j == 0 && (key < it.all_lo || key + kKeys - 1 > it.all_hi)) {
+          settle_values<T, C::kChunks>(smem + C::OFF_KV + (2 * cv + 1) * C::kTile, it.first - key, it.last + 1 - key, it.all_lo - key,
+                                       it.all_hi + 1 - key, &odd[(item_no - 1) & 3], item_no);
         }
         const uint32_t b = v_lo + cv * (2 * kTileLo);
         auto keys64 = [&](int k0, bool first) {
@@ -814,6 +906,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       }
       if (!ok) break;
       const int64_t row = int64_t(it.q0) + tok;
+      if (odd[(item_no - 1) & 3] == item_no) add_odd<T, D, PREFIX>(o_col, recent[(item_no - 1) & 3], p, jlo, jhi);
       if (PREFIX) {
         const int64_t slot = (int64_t(it.z) * p.total_q + row) * p.heads + head;
         if (row_ok) p.part_ml[slot] = make_float2(m, l);
@@ -850,7 +943,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             if (it.n > 0) {
               tmem_ld32(o_col + uint32_t(32 * c), o);
               tmem_wait_ld32(o);
-            } else {
+              } else {
 #pragma unroll
               for (int j = 0; j < 32; ++j) o[j] = 0.f;
             }
@@ -879,7 +972,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             if (it.n > 0) {
               tmem_ld32(o_col + uint32_t(32 * c), o);
               tmem_wait_ld32(o);
-            } else {
+              } else {
 #pragma unroll
               for (int j = 0; j < 32; ++j) o[j] = 0.f;
             }
@@ -984,6 +1077,8 @@ int launch_prefix(const klc_attn_dims& dims, const DecodeParams& d, const void* 
   p.table_stride = d.table_stride;
   p.pages = d.pages;
   p.page_size = d.page_size;
+  p.v = v_pages;
+  p.v_ts = page_stride;
   p.part_o = d.prefix_o;
   p.part_ml = d.prefix_ml;
   CUtensorMap mq, mk, mv;
@@ -1039,6 +1134,9 @@ extern "C" int klc_attn_prompt(const klc_attn_dims* dims, const void* q, int64_t
   p.group = G;
   p.tpt = kRows / G;
   p.scale_log2 = dims->scale * kLog2e;
+  p.v = v;
+  p.v_ts = v_token_stride;
+  p.v_hs = v_head_stride;
   p.window = std::min(dims->window, 1 << 30);  // no position is larger, and position - window stays in 32 bits
   p.sinks = sinks;
   p.out = out;

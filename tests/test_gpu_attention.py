@@ -185,15 +185,56 @@ def test_prompt_keys_that_no_row_sees_may_hold_anything(d, heads, lq, lk, window
     assert torch.equal(attn_prompt(q, k, v, cum(lq), cu_seqlens_k=cum(lk), window=window), clean)
 
 
-def test_prompt_later_values_do_not_reach_earlier_row_tiles():
-    """A value that is not finite reaches rows from its own on, and at most the rows of its own two row tiles before it."""
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("heads,kv,d", [(16, 2, 64), (2, 2, 64), (12, 4, 128), (1, 1, 128)])
+@pytest.mark.parametrize("window", [0, 40, 150])
+@pytest.mark.parametrize("lq,lk", [([400], [400]), ([60, 70], [300, 128]), ([50], [20])])
+def test_prompt_values_that_are_not_finite_reach_the_rows_that_see_them(dtype, heads, kv, d, window, lq, lk):
+    """Bad elements at the diagonal, at tile edges and at window edges: their column of the rows that see the key, nothing else."""
     from kcapw_klcquant_b200 import attn_prompt
 
-    q, k, v = rnd((400, 16, 64), BF, 12), rnd((400, 2, 64), BF, 13), rnd((400, 2, 64), BF, 14)
-    clean = attn_prompt(q, k, v, cum([400]))
-    v[200] = float("nan")
-    got = attn_prompt(q, k, v, cum([400]))
-    assert got[200:].isnan().all() and torch.equal(got[:192], clean[:192])  # 8 heads a key head: 16 tokens a row tile
+    q, k, v = rnd((sum(lq), heads, d), dtype, 12), rnd((sum(lk), kv, d), dtype, 13), rnd((sum(lk), kv, d), dtype, 14)
+    clean = attn_prompt(q, k, v, cum(lq), cu_seqlens_k=cum(lk), window=window)
+    bad = [(lk[0] - 1, 3, float("nan")), (lk[0] // 2, 5, float("inf")), (lk[0] // 2, 40, float("-inf")), (0, 6, float("inf")),
+           (min(127, lk[0] - 1), d - 1, float("nan")), (max(0, lk[0] - 20), 7, float("-inf")), (max(0, lk[0] - 45), 8, float("nan"))]
+    for key, col, val in bad:
+        v[key, kv - 1, col] = val
+    got = attn_prompt(q, k, v, cum(lq), cu_seqlens_k=cum(lk), window=window)
+    want = clean.clone()
+    pos = torch.arange(lq[0], device=DEV) + lk[0] - lq[0]
+    g = heads // kv
+    for key, col, val in bad:
+        see = (pos >= key) & ((pos < key + window) if window else True)
+        want[:lq[0]][see, heads - g:, col] = val
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (HF, 128)])
+def test_decode_prefix_values_that_are_not_finite(dtype, d):
+    """In a shared prefix under a window, a bad value reaches the rows whose window holds its key."""
+    from kcapw_klcquant_b200 import attn_decode
+
+    prefix, window, tails = 320, 200, [1, 30, 90, 150, 199, 260]
+    pk, pv = rnd((prefix, 2, d), dtype, 1), rnd((prefix, 2, d), dtype, 2)
+    ks = [torch.cat([pk, rnd((t, 2, d), dtype, 10 + t)]) for t in tails]
+    vs = [torch.cat([pv, rnd((t, 2, d), dtype, 500 + t)]) for t in tails]
+    q = rnd((len(tails), 8, d), dtype, 3)
+    ln = torch.tensor([prefix + t for t in tails], dtype=torch.int32, device=DEV)
+    gs, pl = torch.tensor([0, len(tails)], dtype=torch.int32, device=DEV), torch.tensor([prefix], dtype=torch.int32, device=DEV)
+
+    def run():
+        kp, vp, table = ref.paged(ks, vs, 32)
+        return attn_decode(q, kp, vp, table, ln, window=window, group_starts=gs, prefix_lens=pl)
+
+    clean = run()
+    want = clean.clone()
+    for key, col, val in ((200, 4, float("nan")), (319, 9, float("inf")), (130, 11, float("nan")), (100, 20, float("inf"))):
+        for i, t in enumerate(tails):
+            vs[i][key, 0, col] = val
+            if key >= prefix + t - window:
+                want[i, :4, col] = val
+    got = run()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
 
 
 def test_prompt_nan_key_is_a_nan_row():
