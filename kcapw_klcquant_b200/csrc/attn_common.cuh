@@ -50,10 +50,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // (in units of log2), the sum l of 2^(s - m) and the unnormalised output.
 // Joining shares k: m = max m_k, l = sum l_k 2^(m_k - m), o likewise.  An
 // attention sink is one more key of weight 2^sink without a value.
-struct RowStats {
-  float m, l;
-};
-
+//
 // 1 / denominator and the log-sum-exp (natural log) of a finished row whose
 // keys gave (m, l), with the head's sink when there is one.  A row that sees
 // no key has l = 0: its output is 0 and its log-sum-exp the sink's (or -inf).

@@ -154,16 +154,17 @@ class MoeStack:
         if self.attention is None:
             raise RuntimeError("the stack has no attention layers")
         T, dev = int(hidden.shape[0]), hidden.device
-        if rows.dim() != 1 or cu_seqlens.shape != (rows.shape[0] + 1,):
-            raise ValueError("cu_seqlens must have one element more than rows")
-        lens = cu_seqlens[1:] - cu_seqlens[:-1]
-        add = torch.zeros_like(self._add)
-        add[rows.long()] = lens
-        self.cache.reserve(add)
+        if rows.dim() != 1 or rows.shape[0] == 0 or cu_seqlens.shape != (rows.shape[0] + 1,):
+            raise ValueError("rows must not be empty and cu_seqlens have one element more")
+        if rows.dtype != torch.int32 or cu_seqlens.dtype != torch.int32 or rows.device != dev or cu_seqlens.device != dev:
+            raise ValueError(f"rows and cu_seqlens must be int32 on {dev}")
+        # by comparison, not by index: a row that does not exist reserves nothing (and is reported), where an index would trap
+        here = torch.arange(self.cache.rows, dtype=torch.int32, device=dev)[:, None] == rows
+        self.cache.reserve((here * (cu_seqlens[1:] - cu_seqlens[:-1])).sum(1, dtype=torch.int32))
         # tokens past the last sequence are padding: row -1
         seq = torch.bucketize(torch.arange(T, dtype=torch.int32, device=dev), cu_seqlens[1:], right=True, out_int32=True)
         inside = seq < rows.shape[0]
-        at = seq.clamp(max=max(rows.shape[0] - 1, 0)).long()
+        at = seq.clamp(max=rows.shape[0] - 1).long()
         positions = torch.arange(T, dtype=torch.int32, device=dev) - cu_seqlens[at]
         token_rows = torch.where(inside, rows[at], -1).to(torch.int32)
         return self._layers(hidden, lambda li, x: self.attention[li].prompt(x, self.cache, li, self.rope, cu_seqlens, positions,

@@ -360,7 +360,16 @@ def test_stack_refusals():
     x = torch.zeros(3, 256, dtype=torch.bfloat16, device=DEV)
     with pytest.raises(ValueError):
         stack.step(x)
-    with pytest.raises(ValueError):
-        stack.prompt(x, i32([0, 3]), i32([0, 1]))
+    for cu, rows in ((i32([0, 3]), i32([0, 1])), (i32([0]), i32([])), (i32([0, 3]).long(), i32([0])), (i32([0, 3]), torch.zeros(1, device=DEV)),
+                     (torch.tensor([0, 3], dtype=torch.int32), i32([0]))):
+        with pytest.raises(ValueError):
+            stack.prompt(x, cu, rows)
+    from kcapw_klcquant_b200 import KlcError
+
+    for rows in ([5], [-3], [2 ** 31 - 1]):  # rows that do not exist: reported, nothing written
+        stack.prompt(x, i32([0, 3]), i32(rows))
+        with pytest.raises(KlcError):
+            stack.cache.check()
+        assert stack.cache.lens.tolist() == [0, 0] and (stack.cache.pool == 0).all()
     with pytest.raises(RuntimeError):
         MoeStack(stack.layers, stack.norm_weights).prompt(x, i32([0, 3]), i32([0]))
