@@ -46,10 +46,23 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// Maxima that keep a NaN: a row with a score that is not a number must not pass for one without keys.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // A row's share of the softmax over some of its keys: the running maximum m
 // (in units of log2), the sum l of 2^(s - m) and the unnormalised output.
 // Joining shares k: m = max m_k, l = sum l_k 2^(m_k - m), o likewise.  An
-// attention sink is one more key of weight 2^sink without a value.
+// attention sink is one more key of weight 2^sink without a value.  m = -inf
+// says that the share has no key: a NaN score makes m or l a NaN, never that.
 //
 // 1 / denominator and the log-sum-exp (natural log) of a finished row whose
 // keys gave (m, l), with the head's sink when there is one.  A row that sees

@@ -343,10 +343,10 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         for (int h = 0; h < 2; ++h) {  // rows `row` and `row + 8`
           float mx = sc[0][2 * h];
 #pragma unroll
-          for (int c = 0; c < 2 * NG; ++c) mx = fmaxf(mx, fmaxf(sc[c][2 * h], sc[c][2 * h + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * p.scale_log2;
-          if (mx > m[h]) {
+          for (int c = 0; c < 2 * NG; ++c) mx = max3_nan(mx, sc[c][2 * h], sc[c][2 * h + 1]);
+          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * p.scale_log2;
+          if (!(mx <= m[h])) {  // larger, or a NaN on either side: l and o become NaN then, and stay so
             const float f = exp2_approx(m[h] - mx);  // 0 from the initial -inf
             m[h] = mx;
             l[h] *= f;
@@ -397,7 +397,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       for (int h = 0; h < 2; ++h) {
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w * kRowTile + row + 8 * h].x);
+        for (int w = 0; w < 4; ++w) top = max_nan(top, ml[w * kRowTile + row + 8 * h].x);
         f[h] = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - top);
       }
       for (int w = 0; w < 4; ++w) {
@@ -426,7 +426,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const int rr = idx / kPerRow, c8 = idx - rr * kPerRow;
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w * kRowTile + rr].x);
+        for (int w = 0; w < 4; ++w) top = max_nan(top, ml[w * kRowTile + rr].x);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const float2 a = ml[w * kRowTile + rr];

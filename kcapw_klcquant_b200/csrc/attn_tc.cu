@@ -173,12 +173,6 @@ __device__ __forceinline__ void tmem_wait_ld64(float* v) {
                : "memory");
 }
 
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
 // pairs of fp32 in one instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;

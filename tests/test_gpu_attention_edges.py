@@ -1,0 +1,63 @@
+"""Attention where the inputs are not finite, the numerators small, the pages gone or the calls unusual: against the definition."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests import attention_ref as ref
+from tests.test_gpu_attention import BF, DEV, HF, check_decode, decode_case, rnd
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+# ---- scores that are not finite --------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,heads,kv,d", [(BF, 64, 8, 64), (HF, 6, 2, 128), (BF, 20, 1, 64)])
+@pytest.mark.parametrize("lens", [[777], [1], [40, 3000, 0, 130, 64], [90] * 200])
+@pytest.mark.parametrize("sink", [False, True])
+def test_decode_nan_query_is_a_nan_row(dtype, heads, kv, d, lens, sink):
+    """Whether the row's keys are cut over many thread blocks or not; its neighbours keep their bits."""
+    from kcapw_klcquant_b200 import attn_decode
+
+    q, ks, vs, sinks = decode_case(dtype, heads, kv, d, lens, 32, 0, sink)
+    kp, vp, table = ref.paged(ks, vs, 32)
+    ln = i32(lens)
+    clean, clean_lse = attn_decode(q, kp, vp, table, ln, sinks=sinks, return_lse=True)
+    hit = torch.zeros(len(lens), heads, dtype=torch.bool, device=DEV)
+    hit[0, 0] = hit[-1, heads - 1] = hit[len(lens) // 2, heads // 2] = True
+    q[..., d - 1][hit] = float("nan")
+    out, lse = attn_decode(q, kp, vp, table, ln, sinks=sinks, return_lse=True)
+    hit &= (ln > 0)[:, None]  # a row without keys has no score to be a NaN
+    assert out[hit].isnan().all() and lse[hit].isnan().all()
+    assert torch.equal(out[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (HF, 128)])
+@pytest.mark.parametrize("keys", [(0, 1), (0, 64), (100, 116), (512, 1024), (0, 3000), (2999, 3000)])
+@pytest.mark.parametrize("window", [0, 200])
+@pytest.mark.parametrize("prefix", [0, 1024])
+def test_decode_nan_keys_make_the_rows_that_see_them_nan(dtype, d, keys, window, prefix):
+    """One key, a warp's, a tile's, a whole share of them: output and log-sum-exp."""
+    from kcapw_klcquant_b200 import attn_decode
+
+    n = 3000
+    q, ks, vs, _ = decode_case(dtype, 8, 2, d, [n, n], 64, 0, False)
+    ks[1][:prefix], vs[1][:prefix] = ks[0][:prefix], vs[0][:prefix]
+    kw = dict(window=window, return_lse=True)
+    if prefix:
+        kw.update(group_starts=i32([0, 2]), prefix_lens=i32([prefix]))
+    ln = i32([n, n])
+    clean, clean_lse = attn_decode(q, *ref.paged(ks, vs, 64), ln, **kw)
+    for k in ks:
+        k[keys[0]:keys[1], 1] = float("nan")
+    out, lse = attn_decode(q, *ref.paged(ks, vs, 64), ln, **kw)
+    assert torch.equal(out[:, :4], clean[:, :4]) and torch.equal(lse[:, :4], clean_lse[:, :4])
+    if window == 0 or keys[1] > n - window:
+        assert out[:, 4:].isnan().all() and lse[:, 4:].isnan().all()
+    else:
+        assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
