@@ -17,11 +17,15 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMaxBatch = 4096;  // sequences per decode call (each CTA keeps 16 bytes of plan per sequence)
 
+// kTopLog2: the softmax numerators are made up to 2^kTopLog2, not up to 1, and the sums carry the same factor.  f16 has
+// 5 exponent bits: with numerators up to 1 those below 2^-14 lose bits and those below 2^-25 vanish, though a long context
+// has many of them (a score 18 below the row's largest is 2^-26), while 2^1 .. 2^15 lie unused.  bf16 has fp32's range.
 template <typename T>
 struct Elem;
 template <>
 struct Elem<__nv_bfloat16> {
   static constexpr uint32_t kMmaFormat = 1;  // tcgen05 kind::f16 operand format field
+  static constexpr float kTopLog2 = 0.f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
@@ -33,6 +37,7 @@ struct Elem<__nv_bfloat16> {
 template <>
 struct Elem<__half> {
   static constexpr uint32_t kMmaFormat = 0;
+  static constexpr float kTopLog2 = 15.f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
@@ -58,8 +63,9 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
-// A row's share of the softmax over some of its keys: the running maximum m
-// (in units of log2), the sum l of 2^(s - m) and the unnormalised output.
+// A row's share of the softmax over some of its keys: a reference m at or
+// below the running maximum (in units of log2), the sum l of 2^(s - m) and the
+// unnormalised output.
 // Joining shares k: m = max m_k, l = sum l_k 2^(m_k - m), o likewise.  An
 // attention sink is one more key of weight 2^sink without a value.  m = -inf
 // says that the share has no key: a NaN score makes m or l a NaN, never that.

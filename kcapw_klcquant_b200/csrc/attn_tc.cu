@@ -17,9 +17,10 @@
 // softmax thread reads its row and writes P as 16-bit pairs, and O += P V
 // reads P from TMEM.  The tensor pipe works on one row tile while the other is
 // in its softmax.  Row statistics are fp32.  O is rescaled only when a row's
-// maximum has grown by more than 2^8 since the last rescale: until then P is at most
-// 2^8, far inside both types' range, and its relative rounding (2^-8 / 2^-11,
-// the price of a 16-bit P operand) does not depend on the reference maximum.
+// maximum has grown by more than 2^8 (f16: 2^4) since the last rescale: until then
+// P is at most 2^8 (f16: 2^15), inside the type's range, and its relative rounding
+// (2^-8 / 2^-11, the price of a 16-bit P operand) does not depend on the reference.
+// f16 keeps that for weights down to 2^-25 of the row's largest; 2^-36 is the smallest that counts.
 //
 // Bound: with D = 128 the chain softmax -> P V -> next S of a row tile (TMEM
 // has no room for a second S), with D = 64 the softmax's instructions.  16221
@@ -76,7 +77,13 @@ constexpr int kThreads = 352;  // 8 softmax warps, an MMA warp for each row tile
 constexpr int kSoftmaxWarps = 8, kWarpMma0 = 8, kWarpTma = 9, kWarpMma1 = 10;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kOutPitch = 80, kOutWarp = 32 * kOutPitch;
-constexpr float kRescaleLog2 = 8.f;
+// A row's reference moves when its maximum has grown by more than 2^kRescale since; it is put 2^kBelow under that maximum,
+// so that numerators use f16's range up to 2^15 (bf16: 2^8, no matter).  f16: 2^4 and 2^11; 2^8 would leave 2^7.
+template <typename T>
+struct Ref {
+  static constexpr float kRescale = Elem<T>::kTopLog2 > 0.f ? 4.f : 8.f;
+  static constexpr float kBelow = Elem<T>::kTopLog2 > 0.f ? Elem<T>::kTopLog2 - kRescale : 0.f;
+};
 constexpr int kItems = 2;      // ring of items between the TMA warp and the others
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -771,7 +778,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       const int wlo = __reduce_max_sync(0xffffffffu, row_ok ? jlo : 0), whi = __reduce_min_sync(0xffffffffu, row_ok ? jhi : 0x7fffffff);
       const int head = it.kvh * G + g;
       const float sink = !PREFIX && row_ok && p.sinks != nullptr ? p.sinks[head] * kLog2e : 0.f;  // used at the end
-      float m = -INFINITY, l = 0.f;  // m: reference maximum (log2 units) of the stored P and O
+      float m = -INFINITY, l = 0.f;  // m: reference (log2 units) of the stored P and O
       bool ok = true;
       for (int i = 0; i < it.n; ++i, ++steps) {
         ok = wait_bar_short(s_full(t), steps & 1, ctl, 508);
@@ -824,9 +831,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
         peak(sb);
         peak(sb + 32);
-        const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;
-        // the reference moves when the maximum has grown by more than 2^8 (or to a NaN)
-        const bool grow = row_ok && (m == -INFINITY ? top != -INFINITY : !(top <= m + kRescaleLog2));
+        const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2 - Ref<T>::kBelow;
+        // the reference moves when the maximum has grown by more than 2^kRescale (or to a NaN)
+        const bool grow = row_ok && (m == -INFINITY ? top != -INFINITY : !(top <= m + Ref<T>::kRescale));
         if (__any_sync(0xffffffffu, grow)) {
           const float f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
           if (grow) {

@@ -61,3 +61,32 @@ def test_decode_nan_keys_make_the_rows_that_see_them_nan(dtype, d, keys, window,
         assert out[:, 4:].isnan().all() and lse[:, 4:].isnan().all()
     else:
         assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
+# ---- small numerators ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,d", [(HF, 64), (HF, 128), (BF, 64)])
+@pytest.mark.parametrize("path,n", [("prompt", 5000), ("decode", 131000), ("prefix", 16384 + 70)])
+@pytest.mark.parametrize("gap", [16.0, 18.0, 21.0])
+def test_many_small_weights_behind_one_large(dtype, d, path, n, gap):
+    """A first key whose value is 0 takes almost all of the softmax: what is left comes from the small weights alone.
+
+    f16 numerators go up to 2^15 and the reference is at most 2^4 under the row's maximum, so that what a numerator loses
+    below the type's normal range is 2^-25 / 2^11 = 2^-36 of the largest weight (attention_ref allows 2^-25)."""
+    from kcapw_klcquant_b200 import attn_decode, attn_prompt
+
+    q = torch.ones((1, 2, d), dtype=dtype, device=DEV)
+    k, v = rnd((n, 1, d), dtype, 1, 0.02), 1 + rnd((n, 1, d), dtype, 2, 0.25)
+    k[0], v[0] = gap / d, 0  # the scores of the others: 0, and 0.02 d^0.5 around it
+    if path == "prompt":
+        out = attn_prompt(q, k, v, i32([0, 1]), cu_seqlens_k=i32([0, n]), scale=1.0)
+    elif path == "decode":
+        out = attn_decode(q, *ref.paged([k], [v], 64), i32([n]), scale=1.0)
+    else:
+        out = attn_decode(q, *ref.paged([k], [v], 64), i32([n]), scale=1.0, group_starts=i32([0, 1]), prefix_lens=i32([16384]))
+    want, _, bound = ref.attention(q, k, v, torch.tensor([n - 1], device=DEV), 1.0)
+    if dtype == HF:
+        bound = bound + (2.0 ** -36 - 2.0 ** -25) * n * v.double().abs().amax()
+    assert (want > 4 * bound).all()  # the bound would not pass zeros
+    ref.assert_close(out, want, bound, path)
