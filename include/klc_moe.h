@@ -443,8 +443,9 @@ int klc_locality_route(const klc_locality_config* cfg, const uint16_t* logits, i
  * product with the values, and the output once at the end.  window 0 sees all
  * earlier keys, window w the last w (the own key among them).  sinks: fp32
  * [heads] or NULL, one more logit per head (unscaled) that takes part in the
- * denominator only.  A row that sees no key gives zeros, and -inf (or the
- * sink) as its log-sum-exp.
+ * denominator only.  A row that sees no key, or only keys whose score is -inf,
+ * gives zeros, and -inf (or the sink) as its log-sum-exp; a score that is +inf
+ * or not a number makes output and log-sum-exp of its row not a number.
  *
  * `status`: a device buffer of klc_status_bytes that the caller zeroed once
  * (or NULL).  The first device-side fault is recorded in it

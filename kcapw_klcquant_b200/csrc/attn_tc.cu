@@ -837,7 +837,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         if (__any_sync(0xffffffffu, grow)) {
           const float f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
           if (grow) {
-            m = top;
+            m = top == INFINITY ? __int_as_float(0x7fffffff) : top;  // inf - inf is not a number; the FMA pipe's share would hide it
             l *= f;
           }
           // O is complete behind the previous P V (D = 128: S of this tile was issued behind it)
@@ -936,6 +936,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         tc_fence_after();
       }
       if (!ok) break;
+      if (m == -INFINITY) l = 0.f;  // no key, or scores of -inf alone (the FMA pipe's share of a whole tile is not an exact 0)
       const int64_t row = int64_t(it.q0) + tok;
       if (odd[(item_no - 1) & 3] == item_no) add_odd<T, D, PREFIX>(o_col, recent[(item_no - 1) & 3], p, jlo, jhi);
       if (PREFIX) {

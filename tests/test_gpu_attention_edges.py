@@ -90,3 +90,50 @@ def test_many_small_weights_behind_one_large(dtype, d, path, n, gap):
         bound = bound + (2.0 ** -36 - 2.0 ** -25) * n * v.double().abs().amax()
     assert (want > 4 * bound).all()  # the bound would not pass zeros
     ref.assert_close(out, want, bound, path)
+
+
+# ---- infinite scores -------------------------------------------------------------------
+
+
+def attend(path, q1, k, v, sinks, window=0):
+    """The last token's attention: as the last of a prompt's rows, over the cache, or over the cache with a shared prefix."""
+    from kcapw_klcquant_b200 import attn_decode, attn_prompt
+
+    n, kw = k.shape[0], dict(sinks=sinks, window=window, return_lse=True)
+    if path == "prompt":
+        q = torch.cat([rnd((39, *q1.shape[1:]), q1.dtype, 3), q1])
+        out, lse = attn_prompt(q, k, v, i32([0, 40]), cu_seqlens_k=i32([0, n]), **kw)
+        return out[39:], lse[39:]
+    if path == "prefix":
+        kw.update(group_starts=i32([0, 1]), prefix_lens=i32([n // 2 // 64 * 64]))
+    return attn_decode(q1, *ref.paged([k], [v], 64), i32([n]), **kw)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (BF, 128), (HF, 64), (HF, 128)])
+@pytest.mark.parametrize("path", ["prompt", "decode", "prefix"])
+@pytest.mark.parametrize("sink", [False, True])
+def test_infinite_scores(dtype, d, path, sink):
+    n = 1200
+    q, k, v = rnd((1, 4, d), dtype, 1).abs() + 0.5, rnd((n, 2, d), dtype, 4), rnd((n, 2, d), dtype, 5)
+    sinks = torch.randn(4, device=DEV) if sink else None
+    clean, clean_lse = attend(path, q, k, v, sinks)
+    for j in (0, 130, 131, 390, 648, n - 1):  # +inf: not a number, in the heads that read it
+        bad = k.clone()
+        bad[j, 1, 5] = float("inf")
+        out, lse = attend(path, q, bad, v, sinks)
+        assert out[:, 2:].isnan().all() and lse[:, 2:].isnan().all(), j
+        assert torch.equal(out[:, :2], clean[:, :2]) and torch.equal(lse[:, :2], clean_lse[:, :2])
+    gone = [0, 130, 131, 390, 648, 649, n - 1]  # -inf: as if the key were not there
+    bad = k.clone()
+    bad[gone, 1, 5] = -float("inf")
+    out, lse = attend(path, q, bad, v, sinks)
+    left = torch.ones(n, dtype=torch.bool, device=DEV)
+    left[gone] = False
+    want, wl, bound = ref.attention(q[:, 2:], k[left, 1:], v[left, 1:], torch.tensor([n], device=DEV), d ** -0.5, 0, sinks[2:] if sink else None)
+    ref.assert_close(out[:, 2:], want, bound, "-inf")
+    ref.assert_lse(lse[:, 2:], wl, "-inf")
+    bad[:, 1, 5] = -float("inf")  # nothing else: as a row that sees no key
+    for window in (0, 100):
+        out, lse = attend(path, q, bad, v, sinks, window)
+        assert (out[:, 2:] == 0).all()
+        assert torch.allclose(lse[:, 2:], sinks[2:] if sink else torch.full_like(lse[:, 2:], -float("inf")), rtol=1e-6, atol=1e-6)
