@@ -149,8 +149,10 @@ class MoeStack:
 
     def prompt(self, hidden: torch.Tensor, cu_seqlens: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
         """Whole prompts through every layer: packed tokens bf16 [T, H], sequence b the rows ``cu_seqlens[b]:cu_seqlens[b + 1]``
-        (int32 on the device), into the empty cache rows ``rows`` int32 [B].  Returns [T, H]; ``cache.check()`` tells whether
-        the pages sufficed."""
+        (int32 on the device), into the empty cache rows ``rows`` int32 [B], each listed once.  Returns [T, H].
+
+        A row that holds keys already, is listed twice or does not exist keeps what it has, its sequence's outputs mean nothing,
+        and ``cache.check()`` reports it, as it does when the pages do not suffice."""
         if self.attention is None:
             raise RuntimeError("the stack has no attention layers")
         T, dev = int(hidden.shape[0]), hidden.device
@@ -160,7 +162,13 @@ class MoeStack:
             raise ValueError(f"rows and cu_seqlens must be int32 on {dev}")
         # by comparison, not by index: a row that does not exist reserves nothing (and is reported), where an index would trap
         here = torch.arange(self.cache.rows, dtype=torch.int32, device=dev)[:, None] == rows
-        self.cache.reserve((here * (cu_seqlens[1:] - cu_seqlens[:-1])).sum(1, dtype=torch.int32))
+        # positions count from 0: in a row with keys they would fall on those, on pages it shares among them.  reserve reports a
+        # negative growth and leaves the row; its tokens become padding
+        times = here.sum(1, dtype=torch.int32)
+        taken = (times > 0) & ((self.cache.lens != 0) | (times > 1))
+        grow = (here * (cu_seqlens[1:] - cu_seqlens[:-1])).sum(1, dtype=torch.int32)
+        self.cache.reserve(torch.where(taken, -1, grow))
+        rows = torch.where((here & taken[:, None]).any(0), -1, torch.where(rows < 0, -2, rows))  # -2: reported, -1: padding
         # tokens past the last sequence are padding: row -1
         seq = torch.bucketize(torch.arange(T, dtype=torch.int32, device=dev), cu_seqlens[1:], right=True, out_int32=True)
         inside = seq < rows.shape[0]

@@ -137,3 +137,69 @@ def test_infinite_scores(dtype, d, path, sink):
         out, lse = attend(path, q, bad, v, sinks, window)
         assert (out[:, 2:] == 0).all()
         assert torch.allclose(lse[:, 2:], sinks[2:] if sink else torch.full_like(lse[:, 2:], -float("inf")), rtol=1e-6, atol=1e-6)
+
+
+# ---- whole layers ----------------------------------------------------------------------
+
+
+def test_prompt_into_a_row_with_keys_is_reported_and_writes_nothing():
+    """After a fork such a row shares its pages: parent and siblings keep their keys, the other prompts of the call are served."""
+    from kcapw_klcquant_b200 import KlcError
+    from tests.test_gpu_kv_cache import make_stack
+
+    stack, alone = make_stack(5, 40, layers=2), make_stack(5, 40, layers=2)
+    cache = stack.cache
+    x = rnd((50, 256), BF, 1)
+    stack.prompt(x[:40], i32([0, 40]), i32([1]))
+    cache.fork(i32([1]), i32([2]))
+    cache.check()
+
+    def state():
+        live = cache.refs > 0
+        return cache.lens.tolist(), cache.block_table[:3].tolist(), cache.pool[:, :, live].clone()
+
+    for rows in ([1], [2]):
+        before = state()
+        stack.prompt(x[:20], i32([0, 20]), i32(rows))
+        with pytest.raises(KlcError):
+            cache.check()
+        after = state()
+        assert after[:2] == before[:2] and torch.equal(after[2], before[2])
+    before = state()
+    out = stack.prompt(x, i32([0, 10, 30, 50]), i32([2, 3, 1]))  # the one in the middle goes to an empty row
+    with pytest.raises(KlcError):
+        cache.check()
+    want = alone.prompt(x[10:30], i32([0, 20]), i32([3]))
+    assert torch.equal(out[10:30], want)
+    assert cache.lens.tolist() == [0, 40, 40, 20, 0] and cache.block_table[:3].tolist() == before[1]
+    for r in (1, 2):
+        held = cache.block_table[r, :3].long()
+        assert torch.equal(cache.pool[:, :, held], alone_pages(x[:40])), r
+    # the same row twice
+    stack.prompt(x[:30], i32([0, 20, 30]), i32([4, 4]))
+    with pytest.raises(KlcError):
+        cache.check()
+    assert cache.lens.tolist() == [0, 40, 40, 20, 0]
+
+
+def alone_pages(x):
+    """The pages a prompt of these tokens fills in a stack of its own."""
+    from tests.test_gpu_kv_cache import make_stack
+
+    stack = make_stack(5, 40, layers=2)
+    stack.prompt(x, i32([0, x.shape[0]]), i32([1]))
+    return stack.cache.pool[:, :, stack.cache.block_table[1, :3].long()]
+
+
+def test_prompt_reports_rows_that_do_not_exist():
+    from kcapw_klcquant_b200 import KlcError
+    from tests.test_gpu_kv_cache import make_stack
+
+    stack = make_stack(2, 20, layers=1)
+    x = rnd((7, 256), BF, 1)
+    for rows in ([0, -1], [0, 2], [0, -2 ** 31]):
+        stack.prompt(x, i32([0, 4, 7]), i32(rows))
+        with pytest.raises(KlcError):
+            stack.cache.check()
+        assert stack.cache.lens.tolist() == [4, 0]
+        stack.cache.free(i32([0]))
