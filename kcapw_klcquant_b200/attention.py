@@ -24,7 +24,7 @@ import threading
 import torch
 
 from . import _lib
-from .moe import _WORKSPACES, as_bf16, workspace
+from .moe import as_bf16
 
 # the current stream of a device as an integer, without making a Stream object for it where torch offers that
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _lib.stream_ptr)
@@ -226,13 +226,19 @@ def attn_prompt(
     return (o, lse) if return_lse else o
 
 
-def _workspace(device: torch.device, nbytes: int, stream: int) -> torch.Tensor:
+# by (device, stream), apart from the MoE workspaces: those begin with a fault word that is still to be read
+_SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def _scratch(index: int, stream: int, nbytes: int, device: torch.device) -> torch.Tensor:
     """Scratch for one call: the stream's own, or, under capture, memory of the graph (two captured
     graphs never share it, on whichever streams they are replayed)."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    ws = _WORKSPACES.get((device.index, stream))
-    return ws if ws is not None and ws.numel() >= nbytes else workspace(device, nbytes, stream)
+    buf = _SCRATCH.get((index, stream))
+    if buf is None or buf.numel() < nbytes:
+        buf = _SCRATCH[index, stream] = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+    return buf
 
 
 def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype, index: int, d: int) -> tuple[int, int]:
@@ -320,11 +326,13 @@ def attn_decode(
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     L = _lib.lib()
     with on_device(dev) as stream:
-        ws = _workspace(q.device, _decode_bytes(dims.dtype, dims.heads, kv_heads, d, B, groups, dev), stream)
+        nbytes = _decode_bytes(dims.dtype, dims.heads, kv_heads, d, B, groups, dev)
+        status = device_status(dev)
+        ws = _scratch(dev, stream, nbytes, q.device)
         _lib.check(L.klc_attn_decode(
             ctypes.byref(dims), *qa, k_pages.data_ptr(), v_pages.data_ptr(), pages, ps, page_stride, block_table.data_ptr(), width,
             table_stride, ln.data_ptr(), B, _lib.ptr(gs), _lib.ptr(pl), groups, _lib.ptr(sk), *oa, _lib.ptr(lse), ws.data_ptr(),
-            ws.numel(), _lib.ptr(device_status(dev)), stream))
+            ws.numel(), _lib.ptr(status), stream))
     return (o, lse) if return_lse else o
 
 

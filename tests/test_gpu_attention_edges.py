@@ -203,3 +203,23 @@ def test_prompt_reports_rows_that_do_not_exist():
             stack.cache.check()
         assert stack.cache.lens.tolist() == [4, 0]
         stack.cache.free(i32([0]))
+
+
+# ---- scratch ---------------------------------------------------------------------------
+
+
+def test_decode_leaves_a_moe_fault_to_be_read():
+    """A layer's fault word lies in its stream's MoE workspace: a decode call on the stream does not touch it."""
+    from kcapw_klcquant_b200 import KlcError, MoeLayer, attn_decode
+    from kcapw_klcquant_b200 import synthetic as syn
+
+    dims = syn.LayerDims(experts=16, hidden=256, intermediate=256, top_k=4)
+    layer = MoeLayer.from_tensors(0, syn.make_layer(dims, seed=3, device=DEV), DEV, top_k=4)
+    q, ks, vs, _ = decode_case(BF, 8, 2, 64, [100, 300], 16, 0, False)
+    kp, vp, table = ref.paged(ks, vs, 16)
+    attn_decode(q, kp, vp, table, i32([100, 300]))  # scratch of the size it needs is there
+    idx = i32([[0, 1, 2, 3], [4, 5, 6, 99]])  # no such expert: recorded by the permute, the pair is left out
+    layer.experts_forward(rnd((2, 256), BF, 1), idx, torch.full((2, 4), 0.25, dtype=BF, device=DEV), path="simt")
+    attn_decode(q, kp, vp, table, i32([100, 300]))
+    with pytest.raises(KlcError):
+        layer.check_device_status()
