@@ -226,19 +226,33 @@ def attn_prompt(
     return (o, lse) if return_lse else o
 
 
+class _Scratch:
+    """Scratch of the calls on one stream.  ``lock`` is held while a call is launched: its kernels follow each other in the
+    stream without another thread's call, on the same scratch, between them."""
+
+    __slots__ = ("lock", "buf")
+
+    def __init__(self):
+        self.lock = threading.Lock()
+        self.buf = None
+
+    def get(self, nbytes: int, device: torch.device) -> torch.Tensor:
+        if self.buf is None or self.buf.numel() < nbytes:
+            self.buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        return self.buf
+
+
 # by (device, stream), apart from the MoE workspaces: those begin with a fault word that is still to be read
-_SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
+_SCRATCH: dict[tuple[int, int], _Scratch] = {}
 
 
-def _scratch(index: int, stream: int, nbytes: int, device: torch.device) -> torch.Tensor:
-    """Scratch for one call: the stream's own, or, under capture, memory of the graph (two captured
+def _scratch(index: int, stream: int) -> _Scratch:
+    """The stream's scratch, or, under capture, one of the call's own in the graph's memory (two captured
     graphs never share it, on whichever streams they are replayed)."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    buf = _SCRATCH.get((index, stream))
-    if buf is None or buf.numel() < nbytes:
-        buf = _SCRATCH[index, stream] = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-    return buf
+        return _Scratch()
+    key = (index, stream)
+    return _SCRATCH.get(key) or _SCRATCH.setdefault(key, _Scratch())
 
 
 def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype, index: int, d: int) -> tuple[int, int]:
@@ -328,11 +342,13 @@ def attn_decode(
     with on_device(dev) as stream:
         nbytes = _decode_bytes(dims.dtype, dims.heads, kv_heads, d, B, groups, dev)
         status = device_status(dev)
-        ws = _scratch(dev, stream, nbytes, q.device)
-        _lib.check(L.klc_attn_decode(
-            ctypes.byref(dims), *qa, k_pages.data_ptr(), v_pages.data_ptr(), pages, ps, page_stride, block_table.data_ptr(), width,
-            table_stride, ln.data_ptr(), B, _lib.ptr(gs), _lib.ptr(pl), groups, _lib.ptr(sk), *oa, _lib.ptr(lse), ws.data_ptr(),
-            ws.numel(), _lib.ptr(status), stream))
+        scratch = _scratch(dev, stream)
+        with scratch.lock:
+            ws = scratch.get(nbytes, q.device)
+            _lib.check(L.klc_attn_decode(
+                ctypes.byref(dims), *qa, k_pages.data_ptr(), v_pages.data_ptr(), pages, ps, page_stride, block_table.data_ptr(), width,
+                table_stride, ln.data_ptr(), B, _lib.ptr(gs), _lib.ptr(pl), groups, _lib.ptr(sk), *oa, _lib.ptr(lse), ws.data_ptr(),
+                ws.numel(), _lib.ptr(status), stream))
     return (o, lse) if return_lse else o
 
 

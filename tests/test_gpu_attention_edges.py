@@ -223,3 +223,32 @@ def test_decode_leaves_a_moe_fault_to_be_read():
     attn_decode(q, kp, vp, table, i32([100, 300]))
     with pytest.raises(KlcError):
         layer.check_device_status()
+
+
+def test_decode_calls_of_several_threads_on_one_stream():
+    """Each call's kernels follow each other in the stream: no thread's shares reach another's rows."""
+    import threading
+
+    from kcapw_klcquant_b200 import attn_decode
+
+    lens = [3000, 17, 900, 4000, 1]  # the same for all threads: only the queries differ
+    _, ks, vs, sinks = decode_case(BF, 16, 2, 64, lens, 64, 0, True)
+    kp, vp, table = ref.paged(ks, vs, 64)
+    ln = i32(lens)
+    qs = [rnd((len(lens), 16, 64), BF, 40 + i) for i in range(4)]
+    want = [attn_decode(q, kp, vp, table, ln, sinks=sinks) for q in qs]
+    outs = [[] for _ in qs]
+    start = threading.Barrier(len(qs))
+
+    def work(i):
+        start.wait()
+        for _ in range(200):
+            outs[i].append(attn_decode(qs[i], kp, vp, table, ln, sinks=sinks))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(qs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert [sum(not torch.equal(o, w) for o in got) for got, w in zip(outs, want)] == [0] * len(qs)
