@@ -9,6 +9,7 @@ call waits for the host, and a captured decode step can grow its sequences.
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import torch
 
@@ -25,7 +26,8 @@ class PagedKvCache:
     how many sequences hold a page.  New pages are the free ones with the lowest
     ids, in the order of the requests.  Requests that cannot be met leave their
     row as it was and are reported by :meth:`check`.  The methods take int32
-    tensors on the device; calls on one cache are ordered on one stream.
+    tensors on the device; calls on one cache are ordered on one stream, from
+    whichever threads they come.
     """
 
     def __init__(self, *, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, rows: int, row_pages: int,
@@ -54,6 +56,7 @@ class PagedKvCache:
         n = ctypes.c_size_t(0)
         _lib.check(_lib.lib().klc_kv_workspace_size(ctypes.byref(self._c), ctypes.byref(n)))
         self._ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+        self._lock = threading.Lock()  # a call's kernels follow each other in the stream: they share _ws with other calls'
 
     @property
     def rows(self) -> int:
@@ -71,7 +74,7 @@ class PagedKvCache:
         return t if t.is_contiguous() else t.contiguous()
 
     def _call(self, fn, *args) -> None:
-        with on_device(self.device.index) as stream:
+        with on_device(self.device.index) as stream, self._lock:
             _lib.check(fn(ctypes.byref(self._c), *args, stream))
 
     def reserve(self, add: torch.Tensor) -> None:

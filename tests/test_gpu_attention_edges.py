@@ -252,3 +252,36 @@ def test_decode_calls_of_several_threads_on_one_stream():
         t.join()
     torch.cuda.synchronize()
     assert [sum(not torch.equal(o, w) for o in got) for got, w in zip(outs, want)] == [0] * len(qs)
+
+
+def test_cache_calls_of_several_threads_on_one_stream():
+    """A fork is a plan and the moves it asks for: another thread's plan does not come between them."""
+    import threading
+
+    from kcapw_klcquant_b200 import PagedKvCache
+
+    n = 4
+    cache = PagedKvCache(layers=1, pages=64, page_size=16, kv_heads=1, head_dim=64, rows=2 * n, row_pages=4, device=DEV)
+    cache.reserve(i32([20] * n + [0] * n))
+    cache.check()
+    for r in range(n):
+        cache.pool[:, :, cache.block_table[r, :2].long()] = r + 1
+    parents, children = [i32([r]) for r in range(n)], [i32([n + r]) for r in range(n)]
+    wrong = torch.zeros(n, dtype=torch.int32, device=DEV)
+    start = threading.Barrier(n)
+
+    def work(r):
+        start.wait()
+        for _ in range(100):
+            cache.fork(parents[r], children[r], copy=True)
+            page = cache.block_table.index_select(0, children[r].long())[0, :2].long().clamp(min=0)
+            wrong[r] += (cache.pool.index_select(2, page) != r + 1).any()
+            cache.free(children[r])
+
+    threads = [threading.Thread(target=work, args=(r,)) for r in range(n)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    cache.check()
+    assert wrong.tolist() == [0] * n and cache.lens.tolist() == [20] * n + [0] * n
