@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import threading
 
 import torch
@@ -427,16 +428,19 @@ class AttentionLayer:
             raise ValueError(f"qkv_weight must be [{rows}, hidden], got {tuple(qkv_weight.shape)}")
         if o_weight.shape != (qkv_weight.shape[1], heads * head_dim):
             raise ValueError(f"o_weight must be [{qkv_weight.shape[1]}, {heads * head_dim}], got {tuple(o_weight.shape)}")
-        if kv_heads < 1 or heads % kv_heads != 0 or head_dim not in (64, 128):
-            raise ValueError("heads must be a multiple of kv_heads, head_dim 64 or 128")
+        if kv_heads < 1 or heads < kv_heads or heads % kv_heads != 0 or heads // kv_heads > 64 or head_dim not in (64, 128):
+            raise ValueError("heads must be a multiple of kv_heads (at most 64 times), head_dim 64 or 128")
+        if not 0 <= window < 1 << 31 or not (scale is None or 0 < scale < math.inf):
+            raise ValueError("window must be >= 0 and fit 32 bits, scale finite and > 0")
+        for name, b, n in (("qkv_bias", qkv_bias, rows), ("o_bias", o_bias, qkv_weight.shape[1]), ("sinks", sinks, heads)):
+            if b is not None and b.shape != (n,):
+                raise ValueError(f"{name} must be [{n}], got {tuple(b.shape)}")
         dev = qkv_weight.device
         self.heads, self.kv_heads, self.head_dim, self.window, self.scale = int(heads), int(kv_heads), int(head_dim), int(window), scale
         self.qkv_weight, self.o_weight = as_bf16(qkv_weight, dev), as_bf16(o_weight, dev)
         self.qkv_bias = None if qkv_bias is None else as_bf16(qkv_bias, dev)
         self.o_bias = None if o_bias is None else as_bf16(o_bias, dev)
         self.sinks = None if sinks is None else sinks.to(device=dev, dtype=torch.float32).contiguous()
-        if self.sinks is not None and self.sinks.shape != (heads,):
-            raise ValueError(f"sinks must be [{heads}]")
 
     @classmethod
     def from_tensors(cls, layer_idx: int, tensors: dict[str, torch.Tensor], device, heads: int, kv_heads: int, head_dim: int,
@@ -452,8 +456,19 @@ class AttentionLayer:
         parts = [get(f"{n}_proj.bias") for n in "qkv"]
         if any(b is None for b in parts) and not all(b is None for b in parts):
             raise ValueError("q, k and v must all have a bias or none")
-        return cls(torch.cat([get(f"{n}_proj.weight") for n in "qkv"]), get("o_proj.weight"), heads, kv_heads, head_dim,
+        weights = [tensors[f"{p}.{n}_proj.weight"].to(dev) for n in "qkvo"]
+        return cls(torch.cat(weights[:3]), weights[3], heads, kv_heads, head_dim,
                    qkv_bias=None if parts[0] is None else torch.cat(parts), o_bias=get("o_proj.bias"), sinks=get("sinks"), window=window)
+
+    def check_cache(self, cache, rope: tuple[torch.Tensor, torch.Tensor]) -> None:
+        """Raise unless the pages of ``cache`` and the rotary tables fit this layer."""
+        dev, pool = self.qkv_weight.device, cache.pool
+        want = (self.kv_heads, self.head_dim)
+        if pool.dtype is not torch.bfloat16 or (pool.shape[3], pool.shape[5]) != want or pool.device != dev:
+            raise ValueError(f"the layer writes bf16 keys of {want[0]} heads of {want[1]} on {dev}, the cache holds {pool.dtype} "
+                             f"of {pool.shape[3]} heads of {pool.shape[5]} on {pool.device}")
+        if len(rope) != 2 or rope[0].shape != rope[1].shape or rope[0].dim() != 2 or 2 * rope[0].shape[1] != self.head_dim:
+            raise ValueError(f"the rotary tables must both be [max_pos, {self.head_dim // 2}]")
 
     def project(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """q [T, heads, D], k and v [T, kv_heads, D] of x bf16 [T, H]: slices of one product."""

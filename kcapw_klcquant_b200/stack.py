@@ -54,6 +54,12 @@ class MoeStack:
                 raise ValueError("one attention layer and one input norm per layer")
             if cache.pool.shape[0] < len(layers):
                 raise ValueError("the cache has fewer layers than the stack")
+            width = input_norm_weights[0].numel()
+            for layer, moe, norms in zip(attention, layers, zip(input_norm_weights, norm_weights)):
+                layer.check_cache(cache, rope)
+                moe_width = moe.hidden if isinstance(moe, MoeLayer) else moe.backend.local.hidden
+                if {layer.qkv_weight.shape[1], moe_width, *(w.numel() for w in norms)} != {width}:
+                    raise ValueError(f"attention, MoE layers and norms must all have {width} columns")
             if fuse_router:
                 raise ValueError("fuse_router routes the next layer's input before its attention: not with attention")
         self.layers = list(layers)
@@ -139,8 +145,15 @@ class MoeStack:
                 hidden, _, normed = layer.forward(post, precision=self.precision, residual=hidden, next_norm=nxt)
         return hidden
 
+    def _check_hidden(self, hidden: torch.Tensor) -> None:
+        """Before lengths advance: a call that raises later would leave rows with lengths that have no keys."""
+        width, dev = self.input_norm_weights[0].numel(), self.cache.device
+        if hidden.dim() != 2 or hidden.shape[1] != width or hidden.dtype != torch.bfloat16 or hidden.device != dev:
+            raise ValueError(f"hidden must be bf16 [tokens, {width}] on {dev}, got {hidden.dtype} {tuple(hidden.shape)} on {hidden.device}")
+
     def _decode_step(self, hidden: torch.Tensor) -> torch.Tensor:
         cache = self.cache
+        self._check_hidden(hidden)
         if hidden.shape[0] != cache.rows:
             raise ValueError(f"a step takes one token for each of the cache's {cache.rows} rows")
         positions = cache.lens.clone()
@@ -155,6 +168,7 @@ class MoeStack:
         and ``cache.check()`` reports it, as it does when the pages do not suffice."""
         if self.attention is None:
             raise RuntimeError("the stack has no attention layers")
+        self._check_hidden(hidden)
         T, dev = int(hidden.shape[0]), hidden.device
         if rows.dim() != 1 or rows.shape[0] == 0 or cu_seqlens.shape != (rows.shape[0] + 1,):
             raise ValueError("rows must not be empty and cu_seqlens have one element more")

@@ -285,3 +285,42 @@ def test_cache_calls_of_several_threads_on_one_stream():
         t.join()
     cache.check()
     assert wrong.tolist() == [0] * n and cache.lens.tolist() == [20] * n + [0] * n
+
+
+def test_stack_refuses_a_cache_that_does_not_fit_and_keeps_lengths_on_bad_inputs():
+    from kcapw_klcquant_b200 import PagedKvCache
+    from kcapw_klcquant_b200.stack import MoeStack
+    from tests.test_gpu_kv_cache import make_stack
+
+    stack = make_stack(2, 20, layers=1)  # 2 key heads of 64, bf16
+    kw = dict(attention=stack.attention, input_norm_weights=stack.input_norm_weights, cache=stack.cache, rope=stack.rope)
+    size = dict(layers=1, pages=4, page_size=16, kv_heads=2, head_dim=64, rows=2, row_pages=2, device=DEV)
+    for bad in (dict(dtype=HF), dict(kv_heads=1), dict(head_dim=128)):
+        with pytest.raises(ValueError):
+            MoeStack(stack.layers, stack.norm_weights, **dict(kw, cache=PagedKvCache(**dict(size, **bad))))
+    cos, sin = stack.rope
+    for rope in ((cos[:, :16], sin[:, :16]), (cos, sin[:9]), (cos,), (cos[0], sin[0])):
+        with pytest.raises(ValueError):
+            MoeStack(stack.layers, stack.norm_weights, **dict(kw, rope=rope))
+    with pytest.raises(ValueError):
+        MoeStack(stack.layers, stack.norm_weights, **dict(kw, input_norm_weights=[torch.ones(128, dtype=BF, device=DEV)]))
+    for x in (torch.zeros(2, 256, device=DEV), torch.zeros(2, 128, dtype=BF, device=DEV), torch.zeros(512, dtype=BF, device=DEV),
+              torch.zeros(2, 256, dtype=BF)):
+        with pytest.raises(ValueError):
+            stack.step(x)
+        with pytest.raises(ValueError):
+            stack.prompt(x, i32([0, 2]), i32([0]))
+        assert stack.cache.lens.tolist() == [0, 0] and int(stack.cache.refs.sum()) == 0
+
+
+@pytest.mark.parametrize("bad", [dict(qkv_bias=5), dict(o_bias=5), dict(sinks=3), dict(window=-1), dict(scale=0.0), dict(scale=float("nan")),
+                                 dict(heads=130, kv_heads=2), dict(heads=0), dict(heads=7), dict(head_dim=80)])
+def test_attention_layer_refuses_what_its_calls_would(bad):
+    from kcapw_klcquant_b200 import AttentionLayer
+
+    a = dict(heads=8, kv_heads=2, head_dim=64, **{k: torch.zeros(v, device=DEV) if k in ("qkv_bias", "o_bias", "sinks") else v for k, v in bad.items()
+                                                 if k not in ("heads", "kv_heads", "head_dim")})
+    a.update({k: v for k, v in bad.items() if k in ("heads", "kv_heads", "head_dim")})
+    w = torch.zeros((a["heads"] + 2 * a["kv_heads"]) * a["head_dim"], 32, device=DEV)
+    with pytest.raises(ValueError):
+        AttentionLayer(w, torch.zeros(32, a["heads"] * a["head_dim"], device=DEV), **a)
