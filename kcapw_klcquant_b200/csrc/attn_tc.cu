@@ -396,6 +396,16 @@ __device__ __noinline__ void add_odd(uint32_t o_col, const Item& it, const TcPar
   tmem_wait_st();
 }
 
+// Whether one of `rows` rows sees a key, of the prefix's `keys`, in the page that starts at `key`: windows of rows of very
+// different lengths leave pages between them that no row sees, whose entries may be gone.
+__device__ __noinline__ bool some_row_sees(const int32_t* lens, int rows, int keys, int window, int key, int page_size) {
+  for (int i = 0; i < rows; ++i) {
+    const int len = lens[i];
+    if (min(len, keys) > key && (window > 0 ? max(0, len - window) : 0) < key + page_size) return true;
+  }
+  return false;
+}
+
 // ---------------------------------------------------------------------------
 // PREFIX = false: packed prompts.  PREFIX = true: single-token rows over the pages of their group's prefix, keys
 // split `splits` ways; shares (m, l, o) go to the workspace and are joined by the decode join.
@@ -600,13 +610,15 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
               for (int c = 0; c < C::kChunks; ++c)
                 tma_load_3d(dst + c * (kKeys * 128), map, c * 64, it.kvh, it.k0 + key, kv_full(s));
             } else {
-              // pages past the prefix, and ids that are no page of the pool, read as zeros (coordinate past the end)
+              // pages without a key that some row sees (their entries may be gone), and ids that are no page of the pool, read
+              // as zeros (coordinate past the end)
               for (int j = 0; j < kKeys; j += p.page_size) {
                 int page = int(p.pages);
-                if (key + j < it.kn) {
+                if (key + j <= it.last && key + j + p.page_size > it.first) {
                   page = p.block_table[int64_t(it.q0) * p.table_stride + (key + j) / p.page_size];
                   if (page < 0 || page >= p.pages) {
-                    record_fault(p.status, KLC_ERR_DEVICE_FAULT, 521, page);
+                    if (some_row_sees(p.lens + it.q0 + it.tok0, min(2 * tpt, it.qn - it.tok0), it.kn, p.window, key + j, p.page_size))
+                      record_fault(p.status, KLC_ERR_DEVICE_FAULT, 521, page);
                     page = int(p.pages);
                   }
                 }

@@ -324,3 +324,28 @@ def test_attention_layer_refuses_what_its_calls_would(bad):
     w = torch.zeros((a["heads"] + 2 * a["kv_heads"]) * a["head_dim"], 32, device=DEV)
     with pytest.raises(ValueError):
         AttentionLayer(w, torch.zeros(32, a["heads"] * a["head_dim"], device=DEV), **a)
+
+
+# ---- shared prefixes -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,heads,kv,d", [(BF, 8, 1, 64), (HF, 6, 2, 128)])
+@pytest.mark.parametrize("ps", [16, 32, 64, 128])
+@pytest.mark.parametrize("window,lens", [(300, [1350, 1313, 1400]), (300, [1281, 1280]), (0, [700, 33, 1000]), (5, [640, 700]), (100, [1400, 1390]),
+                                         (0, [0, 1]), (300, [1350, 200, 0, 1300]), (40, list(range(3, 1400, 137)) * 8)])
+def test_prefix_pages_without_a_visible_key_are_not_looked_up(dtype, heads, kv, d, ps, window, lens):
+    """Entries before every row's window, between the windows of rows of different lengths, and past the longest of rows that end
+    inside the prefix, may be anything."""
+    from kcapw_klcquant_b200 import attn_decode, check_device_status
+
+    prefix, n = 1280, max(1281, *lens)
+    k, v = rnd((n, kv, d), dtype, 1), rnd((n, kv, d), dtype, 2)
+    q, sinks = rnd((len(lens), heads, d), dtype, 3), torch.randn(heads, device=DEV)
+    kp, vp, table = ref.paged([k] * len(lens), [v] * len(lens), ps)
+    for e in range(prefix // ps):
+        if not any(m > e * ps and (m - window if window else 0) < (e + 1) * ps for m in lens):
+            table[:, e] = -1 if e % 2 else 10 ** 6
+    out, lse = attn_decode(q, kp, vp, table, i32(lens), window=window, sinks=sinks, group_starts=i32([0, len(lens)]), prefix_lens=i32([prefix]),
+                           return_lse=True)
+    check_device_status(DEV)
+    check_decode(q, [k[:m] for m in lens], [v[:m] for m in lens], window, sinks, out, lse)
