@@ -362,15 +362,15 @@ struct Cfg {
   static constexpr int kSmem = OFF_OUT + (D == 128 ? kSoftmaxWarps * kOutWarp : 0) + 1024;  // + alignment of the swizzled tiles
 };
 
-// Adds to a row's output in TMEM what odd_rows took out of the values: the elements that are not finite of those keys that the
-// row, but not every row of the item, sees (a positive weight times an infinity or a NaN is that).
+// Adds to a row's output in TMEM what odd_rows took out of the values: the elements that are not finite of those keys of the
+// item's tiles that the row, but not every row of the item, sees (a positive weight times an infinity or a NaN is that).
 template <typename T, int D, bool PREFIX>
 __device__ __noinline__ void add_odd(uint32_t o_col, const Item& it, const TcParams& p, int jlo, int jhi) {
   for (int c = 0; c < D / 32; ++c) {
     float o[32];
     tmem_ld32(o_col + uint32_t(32 * c), o);
     tmem_wait_ld32(o);
-    for (int j = max(it.first, jlo); j <= min(it.last, jhi); ++j) {
+    for (int j = max(max(it.first, it.lo), jlo); j <= min(min(it.last, it.lo + it.n * kKeys - 1), jhi); ++j) {
       if (j >= it.all_lo && j <= it.all_hi) {
         j = it.all_hi;
         continue;
@@ -557,18 +557,20 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         it.tiles = it.tok0 + tpt < it.qn ? 2 : 1;
         int first, last;  // keys some row of the item sees
         if (PREFIX) {
-          int lo = 0x7fffffff, hi = 0;
+          // over the rows that see keys of the prefix at all: an idle row would make every tile a boundary one
+          int lo_min = 0x7fffffff, lo_max = 0, hi_min = 0x7fffffff, hi_max = -1;
           for (int i = it.tok0 + lane; i < min(it.tok0 + 2 * tpt, it.qn); i += 32) {
-            const int len = p.lens[it.q0 + i];
-            lo = min(lo, len);
-            hi = max(hi, len);
+            const int len = p.lens[it.q0 + i], lo = p.window > 0 ? max(0, len - p.window) : 0, hi = min(len, it.kn) - 1;
+            if (lo > hi) continue;
+            lo_min = min(lo_min, lo);
+            lo_max = max(lo_max, lo);
+            hi_min = min(hi_min, hi);
+            hi_max = max(hi_max, hi);
           }
-          lo = __reduce_min_sync(0xffffffffu, lo);
-          hi = __reduce_max_sync(0xffffffffu, hi);
-          first = p.window > 0 ? max(0, lo - p.window) : 0;
-          last = min(hi, it.kn) - 1;
-          it.all_lo = p.window > 0 ? max(0, hi - p.window) : 0;
-          it.all_hi = min(lo, it.kn) - 1;
+          first = __reduce_min_sync(0xffffffffu, lo_min);
+          last = __reduce_max_sync(0xffffffffu, hi_max);
+          it.all_lo = __reduce_max_sync(0xffffffffu, lo_max);
+          it.all_hi = __reduce_min_sync(0xffffffffu, hi_min);
         } else {
           const int pos = it.kn - it.qn + it.tok0;
           first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
@@ -786,8 +788,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         jlo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
         if (jlo > jhi) jlo = 0x7fffffff, jhi = -1;
       }
-      // the row reaches these tiles whole: rows that are not there do not make a tile a boundary one
-      const int wlo = __reduce_max_sync(0xffffffffu, row_ok ? jlo : 0), whi = __reduce_min_sync(0xffffffffu, row_ok ? jhi : 0x7fffffff);
+      // the row reaches these tiles whole: rows that are not there do not make a tile a boundary one (nor do, in a prefix, rows
+      // that see none of it: they keep m = -inf, a share that the join leaves out whatever its O holds)
+      const bool live = PREFIX ? row_ok && jhi >= 0 : row_ok;
+      const int wlo = __reduce_max_sync(0xffffffffu, live ? jlo : 0), whi = __reduce_min_sync(0xffffffffu, live ? jhi : 0x7fffffff);
       const int head = it.kvh * G + g;
       const float sink = !PREFIX && row_ok && p.sinks != nullptr ? p.sinks[head] * kLog2e : 0.f;  // used at the end
       float m = -INFINITY, l = 0.f;  // m: reference (log2 units) of the stored P and O
@@ -813,7 +817,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             if (!__any_sync(0xffffffffu, ja <= 32 * c + 31 && jb >= 32 * c)) none |= 1u << c;
-            if (__any_sync(0xffffffffu, row_ok && (ja > 32 * c || jb < 32 * c + 31))) part |= 1u << c;
+            if (__any_sync(0xffffffffu, live && (ja > 32 * c || jb < 32 * c + 31))) part |= 1u << c;
           }
           part &= ~none;
         }
@@ -845,7 +849,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         peak(sb + 32);
         const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2 - Ref<T>::kBelow;
         // the reference moves when the maximum has grown by more than 2^kRescale (or to a NaN)
-        const bool grow = row_ok && (m == -INFINITY ? top != -INFINITY : !(top <= m + Ref<T>::kRescale));
+        const bool grow = live && (m == -INFINITY ? top != -INFINITY : !(top <= m + Ref<T>::kRescale));
         if (__any_sync(0xffffffffu, grow)) {
           const float f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
           if (grow) {

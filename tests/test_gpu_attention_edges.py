@@ -349,3 +349,37 @@ def test_prefix_pages_without_a_visible_key_are_not_looked_up(dtype, heads, kv, 
                            return_lse=True)
     check_device_status(DEV)
     check_decode(q, [k[:m] for m in lens], [v[:m] for m in lens], window, sinks, out, lse)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (HF, 64), (BF, 128)])
+@pytest.mark.parametrize("window", [0, 700])
+@pytest.mark.parametrize("bad", [None, "v", "k"])
+def test_prefix_rows_that_see_none_of_it(dtype, d, window, bad):
+    """Idle rows and rows whose window lies behind the prefix, between rows that see it; values and keys that are not finite reach
+    the rows that see them only, from whichever share of the prefix they are in."""
+    from kcapw_klcquant_b200 import attn_decode, check_device_status
+
+    prefix, lens = 3200, [3300, 0, 3201, 4200, 3600, 0, 3200]
+    pk, pv = rnd((prefix, 2, d), dtype, 1), rnd((prefix, 2, d), dtype, 2)
+    ks = [torch.cat([pk, rnd((1000, 2, d), dtype, 10 + i)])[:n] for i, n in enumerate(lens)]
+    vs = [torch.cat([pv, rnd((1000, 2, d), dtype, 50 + i)])[:n] for i, n in enumerate(lens)]
+    q = rnd((len(lens), 16, d), dtype, 3)
+    kw = dict(window=window, group_starts=i32([0, len(lens)]), prefix_lens=i32([prefix]), return_lse=True)
+    clean, clean_lse = attn_decode(q, *ref.paged(ks, vs, 64, fill=0.0), i32(lens), **kw)
+    check_device_status(DEV)
+    check_decode(q, ks, vs, window, None, clean, clean_lse)
+    if bad is None:
+        return
+    key = 2850  # seen by 3300, 3201, 3200 (and by 4200 and 3600 without a window)
+    for t in ks if bad == "k" else vs:
+        t[key:key + 1, 1, 9] = float("nan")
+    out, lse = attn_decode(q, *ref.paged(ks, vs, 64, fill=0.0), i32(lens), **kw)
+    want, want_lse = clean.clone(), clean_lse.clone()
+    for i, n in enumerate(lens):
+        if n > key and (window == 0 or key >= n - window):
+            if bad == "k":
+                want[i, 8:], want_lse[i, 8:] = float("nan"), float("nan")
+            else:
+                want[i, 8:, 9] = float("nan")
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+    assert torch.equal(lse.isnan(), want_lse.isnan()) and torch.equal(lse.nan_to_num(nan=0.0), want_lse.nan_to_num(nan=0.0))
