@@ -531,9 +531,12 @@ int klc_rope_append(const klc_attn_dims* dims, const void* q, int64_t q_token_st
  * sequence; lens int32 [rows], its number of keys.  All on the device, all
  * decisions too: no call synchronises, and every call can be captured.  New
  * pages are the free ones with the lowest ids, given to the requests in list
- * order.  A request that cannot be met (no pages left, a row that does not
- * exist, a length past the table) is recorded in status as
- * KLC_ERR_DEVICE_FAULT and leaves its row as it was; the others are served.
+ * order.  A request that cannot be met is recorded in status as
+ * KLC_ERR_DEVICE_FAULT and leaves its row as it was.  One that is bad by itself
+ * (a row that does not exist, a length past the table) does not touch the
+ * others.  When the free pages do not suffice for one, the later ones of the
+ * call that need pages are refused with it, whatever they need: small requests
+ * do not overtake a large one.  Requests that need no page are served.
  * Calls on one cache are ordered on one stream and share one workspace.     */
 typedef struct klc_kv_cache {
   void* pool;

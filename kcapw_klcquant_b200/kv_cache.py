@@ -25,7 +25,9 @@ class PagedKvCache:
     (-1: none), ``lens`` int32 [rows] its number of keys, ``refs`` int32 [pages]
     how many sequences hold a page.  New pages are the free ones with the lowest
     ids, in the order of the requests.  Requests that cannot be met leave their
-    row as it was and are reported by :meth:`check`.  The methods take int32
+    row as it was and are reported by :meth:`check`; when the free pages do not
+    suffice for one, the later ones of the call that need pages are refused with
+    it (small requests do not overtake a large one).  The methods take int32
     tensors on the device; calls on one cache are ordered on one stream, from
     whichever threads they come.
     """

@@ -383,3 +383,27 @@ def test_prefix_rows_that_see_none_of_it(dtype, d, window, bad):
                 want[i, 8:, 9] = float("nan")
     assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
     assert torch.equal(lse.isnan(), want_lse.isnan()) and torch.equal(lse.nan_to_num(nan=0.0), want_lse.nan_to_num(nan=0.0))
+
+
+# ---- pages -----------------------------------------------------------------------------
+
+
+def test_requests_behind_one_that_runs_out_of_pages():
+    """Refused with it if they need pages, served if they do not; a request that is bad by itself touches no other."""
+    from kcapw_klcquant_b200 import KlcError, PagedKvCache
+
+    cache = PagedKvCache(layers=1, pages=6, page_size=16, kv_heads=1, head_dim=64, rows=5, row_pages=12, device=DEV)
+    cache.reserve(i32([0, 0, 0, 10, 0]))  # one page, six more keys fit
+    cache.check()
+    cache.reserve(i32([160, 16, 1, 3, 0]))
+    with pytest.raises(KlcError):
+        cache.check()
+    assert cache.lens.tolist() == [0, 0, 0, 13, 0] and int(cache.refs.sum()) == 1
+    cache.reserve(i32([-1, 16, 10 ** 6, 3, 1]))
+    with pytest.raises(KlcError):
+        cache.check()
+    assert cache.lens.tolist() == [0, 16, 0, 16, 1] and int(cache.refs.sum()) == 3
+    cache.fork(i32([3, 9, 4, 1, 4]), i32([0, 2, 7, 2, 2]))  # a row twice: the first listing counts, and it is a bad one
+    with pytest.raises(KlcError):
+        cache.check()
+    assert cache.lens.tolist() == [16, 16, 0, 16, 1]
