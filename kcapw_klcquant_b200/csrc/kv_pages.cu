@@ -272,7 +272,10 @@ __global__ void __launch_bounds__(kCopyThreads) kv_free_kernel(const KvParams p,
   __syncthreads();
   const int len = len_s;
   if (!len_ok(p, len)) {
-    if (threadIdx.x == 0) record_fault(p.status, KLC_ERR_DEVICE_FAULT, 536, r);
+    if (threadIdx.x == 0) {
+      p.c.lens[r] = len;  // the row stays as it was
+      record_fault(p.status, KLC_ERR_DEVICE_FAULT, 536, r);
+    }
     return;
   }
   const int held = pages_of(len, p.c.page_size);

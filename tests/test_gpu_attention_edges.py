@@ -407,3 +407,15 @@ def test_requests_behind_one_that_runs_out_of_pages():
     with pytest.raises(KlcError):
         cache.check()
     assert cache.lens.tolist() == [16, 16, 0, 16, 1]
+
+
+def test_free_leaves_a_row_with_a_length_past_its_table():
+    from kcapw_klcquant_b200 import KlcError, PagedKvCache
+
+    cache = PagedKvCache(layers=1, pages=6, page_size=16, kv_heads=1, head_dim=64, rows=3, row_pages=2, device=DEV)
+    cache.reserve(i32([20, 3, 0]))
+    cache.lens[0] = 33  # two pages of 16
+    cache.free(i32([0, 1, 2]))
+    with pytest.raises(KlcError):
+        cache.check()
+    assert cache.lens.tolist() == [33, 0, 0] and cache.refs.tolist() == [1, 1, 0, 0, 0, 0]
