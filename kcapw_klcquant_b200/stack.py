@@ -183,12 +183,12 @@ class MoeStack:
         grow = (here * (cu_seqlens[1:] - cu_seqlens[:-1])).sum(1, dtype=torch.int32)
         self.cache.reserve(torch.where(taken, -1, grow))
         rows = torch.where((here & taken[:, None]).any(0), -1, torch.where(rows < 0, -2, rows))  # -2: reported, -1: padding
-        # tokens past the last sequence are padding: row -1
+        # tokens before the first and past the last sequence are padding: row -1
         seq = torch.bucketize(torch.arange(T, dtype=torch.int32, device=dev), cu_seqlens[1:], right=True, out_int32=True)
         inside = seq < rows.shape[0]
         at = seq.clamp(max=rows.shape[0] - 1).long()
         positions = torch.arange(T, dtype=torch.int32, device=dev) - cu_seqlens[at]
-        token_rows = torch.where(inside, rows[at], -1).to(torch.int32)
+        token_rows = torch.where(inside & (positions >= 0), rows[at], -1).to(torch.int32)
         return self._layers(hidden, lambda li, x: self.attention[li].prompt(x, self.cache, li, self.rope, cu_seqlens, positions,
                                                                             token_rows))
 

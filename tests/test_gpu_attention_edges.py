@@ -419,3 +419,14 @@ def test_free_leaves_a_row_with_a_length_past_its_table():
     with pytest.raises(KlcError):
         cache.check()
     assert cache.lens.tolist() == [33, 0, 0] and cache.refs.tolist() == [1, 1, 0, 0, 0, 0]
+
+
+def test_prompt_tokens_before_the_first_sequence_are_padding():
+    from tests.test_gpu_kv_cache import make_stack
+
+    stack, alone = make_stack(2, 20, layers=2), make_stack(2, 20, layers=2)
+    x = rnd((30, 256), BF, 1)
+    out = stack.prompt(x, i32([4, 4, 21]), i32([0, 1]))
+    stack.cache.check()
+    assert stack.cache.lens.tolist() == [0, 17]
+    assert torch.equal(out[4:21], alone.prompt(x[4:21], i32([0, 17]), i32([1])))
