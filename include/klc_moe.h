@@ -512,9 +512,11 @@ int klc_attn_decode(const klc_attn_dims* dims, const void* q, int64_t q_token_st
  * (both int32 on the device; the pages must be there already: klc_kv_reserve).
  * A token with rows[t] = -1 is padding: nothing is written for it.  q_out may
  * be q; k_out (or NULL) receives the rotated keys as rows too.  Two tokens with
- * the same row and position leave either's key and value.  Rows, positions and
- * page ids out of range are recorded as KLC_ERR_DEVICE_FAULT and the token is
- * skipped.  Strides and pools as for klc_attn_decode.  (apply_rope of
+ * the same row and position leave an unspecified mix of their keys and values.
+ * Rows, positions and page ids out of range are recorded as
+ * KLC_ERR_DEVICE_FAULT and nothing is written into the cache for the token (its
+ * rotated query, where the page alone is bad, is).  Strides and pools as for
+ * klc_attn_decode.  (apply_rope of
  * streamed_attention.py, KVCacheManager's append kv_cache_manager.py:50-66) */
 int klc_rope_append(const klc_attn_dims* dims, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                     int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,

@@ -371,7 +371,8 @@ def rope_append(
     """Rotary embedding of q [T, heads, D] and k [T, kv_heads, D], and the write of k and v into the cache.
 
     Token t is key ``positions[t]`` of sequence ``rows[t]`` (int32 on the device;
-    row -1: padding, nothing is written); its page must be reserved.  ``cos`` and
+    row -1: padding, nothing is written, ``out`` included); its page must be reserved,
+    and no other token of the call may have the same row and position.  ``cos`` and
     ``sin`` are fp32 [max_pos, D / 2]; the halves of a head's row are rotated
     against each other, in fp32, rounded once.  Returns the rotated queries
     (``out``, which may be q), and with ``return_k`` the rotated keys [T, kv_heads, D] too.
@@ -488,7 +489,8 @@ class AttentionLayer:
 
     def decode(self, x: torch.Tensor, cache, layer: int, rope: tuple[torch.Tensor, torch.Tensor], positions: torch.Tensor,
                rows: torch.Tensor, group_starts: torch.Tensor | None = None, prefix_lens: torch.Tensor | None = None) -> torch.Tensor:
-        """One token per sequence (x [rows, H], reserved in ``cache``): writes its key and value, returns [rows, H]."""
+        """One token for every row of ``cache`` (x [rows, H], token r that of row r, reserved): writes its key and value, returns
+        [rows, H].  ``rows[r]`` is r, or -1 for a row that sits out (nothing is written, its output means nothing)."""
         q, k, v = self.project(x)
         q = rope_append(q, k, v, *rope, positions, rows, cache.k(layer), cache.v(layer), cache.block_table)
         o = attn_decode(q, cache.k(layer), cache.v(layer), cache.block_table, cache.lens, window=self.window, sinks=self.sinks,

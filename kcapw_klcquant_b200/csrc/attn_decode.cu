@@ -20,9 +20,10 @@
 //     is not the bound).  Each warp keeps its own running
 //     maximum, sum and 16 x D output; the four are joined once per item.
 //   * Rows of a group share their first keys (the prefix): the tensor-core kernel of attn_tc.cu reads
-//     those once for all rows of the group, this one starts behind them, and the join
-//     adds the prefix's shares.  The two run at the same time (programmatic launch); only the
-//     join waits for both.
+//     those once for all rows of the group, this one takes the keys behind them, and the join
+//     adds the prefix's shares.  This kernel may start beside the prefix kernel (programmatic launch), but not
+//     on the same SMs (195 and 105 KB of shared memory): with a prefix item on every SM it runs as those
+//     finish.  The join waits for both.
 #include <algorithm>
 
 #include "attn_common.cuh"

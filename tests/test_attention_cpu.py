@@ -144,3 +144,25 @@ def test_reference_attention_against_scaled_rows():
         assert torch.allclose(out[i, 0], v.half().double()[:i + 1, 0].mean(0)) and math.isclose(float(lse[i, 0]), math.log(i + 1), abs_tol=1e-12)
     out, _, _ = ref.attention(z.half(), z.half(), v.half(), torch.arange(4), 1.0, window=1, sinks=torch.zeros(1))
     assert torch.allclose(out[:, 0], v.half().double()[:, 0] / 2)
+
+
+@pytest.mark.parametrize("heads,kv,d", [(4, 2, 64), (3, 1, 128)])
+@pytest.mark.parametrize("n,m,window,sink", [(1, 1, 0, False), (70, 70, 0, True), (9, 200, 30, True), (40, 41, 1, False)])
+def test_plain_forms_of_the_cases(heads, kv, d, n, m, window, sink):
+    """Plain and 64-bit form of the benchmark's attention against the tests' own reference (no case has fewer keys than queries, and
+    the plain form divides by nothing there); its rotation against complex products."""
+    from perf import operators as ops
+
+    g = torch.Generator().manual_seed(n + m)
+    q, k, v = torch.randn(n, heads, d, generator=g), torch.randn(m, kv, d, generator=g), torch.randn(m, kv, d, generator=g)
+    sinks = torch.randn(heads, generator=g) if sink else None
+    pos = torch.arange(n) + m - n
+    want, _, _ = ref.attention(q.half(), k.half(), v.half(), pos, 0.3, window, sinks)
+    q, k, v = q.half().float(), k.half().float(), v.half().float()
+    # fp32: sums of d products and of m weights; the definition in 64 bits: to its own rounding
+    assert (ops._plain_attention(q, k, v, m - n, 0.3, window, sinks) - want).abs().max() <= 2e-4
+    assert (ops._exact_attention(q, k, v, m - n, 0.3, window, sinks) - want).abs().max() <= 1e-10
+    assert ops._visible(m - n, m - 1, window) == sum(min(p + 1, window) if window else p + 1 for p in range(m - n, m))
+    ang = torch.rand(n, d // 2, generator=g)
+    turned = torch.view_as_real(torch.complex(*q.chunk(2, -1)) * torch.polar(torch.ones_like(ang), ang)[:, None])
+    assert torch.allclose(ops._rotate(q, ang.cos()[:, None], ang.sin()[:, None]), torch.cat([turned[..., 0], turned[..., 1]], -1), atol=1e-5)
