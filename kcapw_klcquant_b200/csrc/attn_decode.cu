@@ -347,7 +347,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           for (int c = 0; c < 2 * NG; ++c) mx = max3_nan(mx, sc[c][2 * h], sc[c][2 * h + 1]);
           mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * p.scale_log2 - Elem<T>::kTopLog2;  // the largest numerator: 2^kTopLog2
-          if (!(mx <= m[h])) {  // larger, or a NaN on either side: l and o become NaN then, and stay so
+          if (mx > m[h] || mx != mx) {  // a NaN stays: nothing is larger, and a tile without keys must not take its place
             const float f = exp2_approx(m[h] - mx);  // 0 from the initial -inf
             m[h] = mx;
             l[h] *= f;

@@ -859,8 +859,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         peak(sb);
         peak(sb + 32);
         const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2 - Ref<T>::kBelow;
-        // the reference moves when the maximum has grown by more than 2^kRescale (or to a NaN)
-        const bool grow = live && (m == -INFINITY ? top != -INFINITY : !(top <= m + Ref<T>::kRescale));
+        // the reference moves when the maximum has grown by more than 2^kRescale, or to a NaN, and stays there: a tile without
+        // keys must not take its place
+        const bool grow = live && (m == -INFINITY ? top != -INFINITY : top > m + Ref<T>::kRescale || top != top);
         if (__any_sync(0xffffffffu, grow)) {
           const float f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
           if (grow) {

@@ -430,3 +430,28 @@ def test_prompt_tokens_before_the_first_sequence_are_padding():
     stack.cache.check()
     assert stack.cache.lens.tolist() == [0, 17]
     assert torch.equal(out[4:21], alone.prompt(x[4:21], i32([0, 17]), i32([1])))
+
+
+@pytest.mark.parametrize("dtype,heads,kv,d", [(BF, 4, 2, 64), (HF, 34, 2, 128), (HF, 8, 1, 64)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("path", ["prompt", "decode", "prefix"])
+def test_tiles_without_keys_do_not_hide_a_nan_seen_before(dtype, heads, kv, d, value, path):
+    """A score that is not a number, then tiles of which the row (or, in decode, a warp's part of the row) sees nothing."""
+    from kcapw_klcquant_b200 import attn_decode, attn_prompt
+
+    key, q = 100, rnd((300, heads, d), dtype, 1).abs() + 0.1
+    k, v = rnd((700, kv, d), dtype, 2), rnd((700, kv, d), dtype, 3)
+    k[key, kv - 1, 5] = value
+    if path == "prompt":  # rows of one item end in different tiles
+        out, lse = attn_prompt(q, k[:300], v[:300], i32([0, 300]), return_lse=True)
+        hit = torch.arange(300, device=DEV) >= key
+    else:
+        lens = [101 + i % 150 for i in range(300)] if path == "decode" else [90 + 2 * i for i in range(300)]
+        kw = {} if path == "decode" else dict(group_starts=i32([0, 300]), prefix_lens=i32([640]))
+        kp, vp, table = ref.paged([k], [v], 64)
+        out, lse = attn_decode(q, kp, vp, table.expand(300, -1).contiguous(), i32(lens), return_lse=True, **kw)
+        hit = i32(lens) > key
+    group = heads // kv
+    for got in (out, lse):
+        assert got[hit, heads - group:].isnan().all()
+        assert got[~hit].isfinite().all() and got[:, :heads - group].isfinite().all()
