@@ -455,3 +455,67 @@ def test_tiles_without_keys_do_not_hide_a_nan_seen_before(dtype, heads, kv, d, v
     for got in (out, lse):
         assert got[hit, heads - group:].isnan().all()
         assert got[~hit].isfinite().all() and got[:, :heads - group].isfinite().all()
+
+
+# ---- captured, large -------------------------------------------------------------------
+
+
+def test_captured_prefix_decode_serves_other_groups_and_two_graphs_run_side_by_side():
+    from kcapw_klcquant_b200 import attn_decode, check_device_status
+
+    n, prefix = 6, 640
+    k, v = rnd((1400, 2, 64), BF, 1), rnd((1400, 2, 64), BF, 2)
+    kp, vp, table = ref.paged([k], [v], 32)
+    table = table.expand(n, -1).contiguous()
+    q = [rnd((n, 8, 64), BF, 3 + i) for i in range(2)]
+    ln, gs, pl = i32([700] * n), i32([0, 3, 6]), i32([prefix, prefix])
+    attn_decode(q[0], kp, vp, table, ln, group_starts=gs, prefix_lens=pl)
+    graphs = []
+    for x in q:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = attn_decode(x, kp, vp, table, ln, window=900, group_starts=gs, prefix_lens=pl)
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for lens, starts, pres in (([700] * n, [0, 3, 6], [640, 640]), ([1400, 3, 0, 900, 640, 1280], [1, 1, 5], [32, 1248]),
+                               ([641, 642, 643, 1, 1399, 33], [0, 6, 6], [640, 0]), ([1400] * n, [2, 2, 2], [64, 64])):
+        ln.copy_(i32(lens))
+        gs.copy_(i32(starts))
+        pl.copy_(i32(pres))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for s, (g, _) in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        check_device_status(DEV)
+        for x, (_, out) in zip(q, graphs):
+            check_decode(x, [k[:m] for m in lens], [v[:m] for m in lens], 900, None, out, None)
+
+
+def test_pages_past_32_bits():
+    """A pool of 5.2e9 elements whose last pages are the free ones: append, attend, fork with copies, compact."""
+    from kcapw_klcquant_b200 import PagedKvCache, attn_decode, rope_append
+
+    pages, ps, kv, d, n = 20000, 128, 8, 128, 300
+    cache = PagedKvCache(layers=1, pages=pages, page_size=ps, kv_heads=kv, head_dim=d, rows=3, row_pages=4, device=DEV)
+    cache.refs[:pages - 8] = 1
+    cache.reserve(i32([n, 0, 0]))
+    assert cache.block_table[0].tolist() == [pages - 8, pages - 7, pages - 6, -1]
+    q, k, v = rnd((n, 8, d), BF, 1), rnd((n, kv, d), BF, 2), rnd((n, kv, d), BF, 3)
+    ang = torch.arange(n, device=DEV, dtype=torch.float64)[:, None] * 0.01 * torch.arange(d // 2, device=DEV, dtype=torch.float64)
+    q, k = rope_append(q, k, v, ang.cos().float(), ang.sin().float(), torch.arange(n, device=DEV, dtype=torch.int32),
+                       torch.zeros(n, device=DEV, dtype=torch.int32), cache.k(0), cache.v(0), cache.block_table, return_k=True)
+    cache.fork(i32([0, 0]), i32([1, 2]))
+    cache.check()
+
+    def attend():
+        out = attn_decode(q[-3:], cache.k(0), cache.v(0), cache.block_table, cache.lens)
+        check_decode(q[-3:], [k] * 3, [v] * 3, 0, None, out, None)
+
+    attend()
+    cache.refs[:pages - 8] = 0
+    assert int(cache.compact()) == 5
+    cache.check()
+    assert sorted(set(cache.block_table.flatten().tolist())) == [-1, 0, 1, 2, 3, 4]
+    attend()
