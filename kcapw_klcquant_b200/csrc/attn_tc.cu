@@ -24,9 +24,10 @@
 // f16 keeps that for weights down to 2^-25 of the row's largest; 2^-36 is the smallest that counts.
 //
 // Bound: with D = 128 the chain softmax -> P V -> next S of a row tile (TMEM
-// has no room for a second S), with D = 64 the softmax's instructions.  16221
-// tokens, 32 / 8 heads of 128: 2.04 ms, 1.06 PFLOP/s, 62 % of the burst rate of
-// a library product (73 % of its sustained one); 6016 tokens, 64 / 8 heads of
+// has no room for a second S), with D = 64 the latencies of two softmax warps a
+// scheduler (no pipe is full).  16221
+// tokens, 32 / 8 heads of 128: 2.02 ms, 1.07 PFLOP/s, 62 % of the burst rate of
+// a library product (74 % of its sustained one); 6016 tokens, 64 / 8 heads of
 // 64: 408 us, 727 TFLOP/s.
 #include <algorithm>
 #include <type_traits>
