@@ -494,8 +494,10 @@ int klc_attn_prompt(const klc_attn_dims* dims, const void* q, int64_t q_tokens, 
  * serves other lengths on replay.  Results do not depend on timing.  A page id
  * outside [0, pages) and a length outside [0, table_width * page_size] are
  * recorded as KLC_ERR_DEVICE_FAULT.  At most 4096 sequences.  One workspace
- * per call in flight.  Replaces StreamedAttention.forward over the
- * KVCacheManager's list (streamed_attention.py:100-152).                    */
+ * per call in flight, its kernels launched without another call on the same
+ * workspace between them; it holds no fault word (faults go to status), and a
+ * MoE workspace passed here loses its own.  Replaces StreamedAttention.forward
+ * over the KVCacheManager's list (streamed_attention.py:100-152).           */
 int klc_attn_decode_workspace_size(const klc_attn_dims* dims, int64_t batch, int64_t groups, size_t* out_bytes);
 int klc_attn_decode(const klc_attn_dims* dims, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                     const void* k_pages, const void* v_pages, int64_t pages, int page_size, int64_t page_stride,

@@ -519,3 +519,34 @@ def test_pages_past_32_bits():
     cache.check()
     assert sorted(set(cache.block_table.flatten().tolist())) == [-1, 0, 1, 2, 3, 4]
     attend()
+
+
+def test_captured_prompt_serves_other_rows_and_offsets():
+    from kcapw_klcquant_b200 import KlcError
+    from tests.test_gpu_kv_cache import make_stack
+
+    stack, eager = make_stack(4, 40, layers=2), make_stack(4, 40, layers=2)
+    x, cu, rows = rnd((48, 256), BF, 1), i32([0, 20, 48]), i32([1, 3])
+    stack.prompt(x, cu, rows)
+    stack.cache.free(rows)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = stack.prompt(x, cu, rows)
+    for offsets, into in (([0, 20, 48], [1, 3]), ([0, 48, 48], [2, 0]), ([3, 10, 40], [0, 2])):
+        cu.copy_(i32(offsets))
+        rows.copy_(i32(into))
+        x.copy_(rnd((48, 256), BF, 7 + offsets[1]))
+        g.replay()
+        stack.cache.check()
+        want = eager.prompt(x, cu, rows)
+        a, b = offsets[0], offsets[-1]
+        assert torch.equal(out[a:b], want[a:b]) and torch.equal(stack.cache.lens, eager.cache.lens)
+        live = eager.cache.refs > 0
+        assert torch.equal(stack.cache.refs, eager.cache.refs) and torch.equal(stack.cache.pool[:, :, live], eager.cache.pool[:, :, live])
+        if offsets[0]:
+            g.replay()  # the rows hold keys now
+            with pytest.raises(KlcError):
+                stack.cache.check()
+            assert torch.equal(stack.cache.lens, eager.cache.lens)
+        for s in (stack, eager):
+            s.cache.free(rows)
